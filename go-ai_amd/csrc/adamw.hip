@@ -1,0 +1,475 @@
+// adamw.hip -- one AdamW step over many tensors in one launch, the moments in 32 or in 8 bits, and the gradients' global
+// norm with its clipping coefficient.
+//
+//   g' = k g,  k = min(1, max_norm / |g|)      (|g| over all tensors; without clipping k = 1)
+//   m  = b1 m + (1 - b1) g',   v = b2 v + (1 - b2) g'^2
+//   p  = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// All of it is float32, every operation rounded on its own (the library is built with -ffp-contract=off), so that a moment
+// in 8 bits is the same code wherever the step is computed.  The norm is summed in float64: a code next to the border of two
+// would follow the last bit of k.
+//
+// Moments in 8 bits are held in blocks of AW_BLOCK elements (no block spans two tensors) with one float32 scale each:
+//   m: e4m3 codes of m / scale, scale = largest |m| of the block / 448 (half a step: 2^-4 of the value, above 2^-15 of the largest);
+//   v: codes of its root r = sqrt(v), c = 1 .. 255 for the float32 with the bits (c + AW_LEVEL0) << 19 (four exponent and four
+//      fraction bits, the largest r of the block is 1.0 = code 255; half a step: 2^-5 of r), 0 for r = 0.  A root that is not zero
+//      never becomes 0: m / (0 + eps) would throw the parameter away.
+// The update itself uses the moments before they are rounded.  A block whose largest value is below 2^-100 is held as zeros.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "ctx.h"
+#include "elem.h"
+#include "goai_internal.h"
+
+namespace goai {
+
+constexpr int AW_BLOCK = 256;          // elements per scale of an 8-bit moment: four per lane of a wavefront
+constexpr int AW_CHUNK = 2048;         // elements per workgroup
+constexpr int AW_LEVEL0 = 1777;        // (255 + AW_LEVEL0) << 19 is 1.0f
+constexpr float AW_SMALLEST = 0x1p-100f;
+constexpr int AW_LAUNCH = 256;         // tensors per launch: their gradients' addresses travel in the launch's arguments
+constexpr int AW_NORM_BLOCKS = 1024;   // workgroups (and float64 partial sums) of the norm
+
+struct AwTensor {
+    void* p;
+    long start, n;           // first element in the moments' flat arrays (a multiple of AW_BLOCK); elements
+    float decay;
+    int ptype, gtype;        // GOAI_ELEM_*
+};
+struct AwState {             // flat arrays over all tensors: float32, or codes and one scale per block
+    void *m, *v;
+    float *ms, *vs;
+};
+struct AwChunk {
+    int tensor, chunk;
+};
+struct AwGrads {
+    const void* g[AW_LAUNCH];
+};
+struct AwScal {
+    double lr;
+    float b1, omb1, b2, omb2, eps, c1, c2;     // c1 = 1 / sqrt(1 - b2^t), c2 = lr / (1 - b1^t)
+};
+
+}  // namespace goai
+
+struct goai_adamw {
+    int device = 0, bits = 32;
+    long elems = 0;                            // of the moments' flat arrays
+    goai::AwState state{};
+    std::vector<goai::AwTensor> tensors;
+    std::vector<int> first;                    // first chunk of each tensor (and the total)
+    goai::AwTensor* d_tensors = nullptr;
+    goai::AwChunk* d_chunks = nullptr;
+    double* d_partials = nullptr;              // AW_NORM_BLOCKS
+};
+
+namespace goai {
+
+// four neighbouring elements from i on, as floats (zeros from `n` on); tensors are aligned to their element type only
+template <int E> __device__ __forceinline__ void aw_load(const void* base, long i, long n, float (&out)[4])
+{
+    using raw = typename Elem<E>::raw;
+    const raw* q = (const raw*)base + i;
+    for (int k = 0; k < 4; k++) out[k] = i + k < n ? elem_to_float<E>(q[k]) : 0.0f;
+}
+template <int E> __device__ __forceinline__ void aw_store(void* base, long i, long n, const float (&x)[4])
+{
+    using raw = typename Elem<E>::raw;
+    raw* q = (raw*)base + i;
+    for (int k = 0; k < 4; k++)
+        if (i + k < n) q[k] = elem_from_float<E>(x[k]);
+}
+
+__device__ __forceinline__ float aw_wave_max(float x)
+{
+    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+
+// ---- moments in 8 bits: four neighbouring codes per lane, a block per wavefront ----
+__device__ __forceinline__ void aw_mean_of(unsigned code, float scale, float (&m)[4])
+{
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(code, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
+    m[0] = lo[0] * scale;
+    m[1] = lo[1] * scale;
+    m[2] = hi[0] * scale;
+    m[3] = hi[1] * scale;
+}
+__device__ __forceinline__ void aw_root_of(unsigned code, float scale, float (&r)[4])
+{
+    for (int k = 0; k < 4; k++) {
+        const unsigned c = (code >> (8 * k)) & 255u;
+        r[k] = c ? __uint_as_float((c + AW_LEVEL0) << 19) * scale : 0.0f;
+    }
+}
+__device__ __forceinline__ unsigned aw_pack_mean(const float (&m)[4], float& scale)
+{
+    const float big = aw_wave_max(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
+    const bool held = big >= AW_SMALLEST;
+    const float inv = held ? (1.0f / big) * 448.0f : 0.0f;
+    scale = held ? big * (1.0f / 448.0f) : 0.0f;
+    int code = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * inv, m[1] * inv, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(m[2] * inv, m[3] * inv, code, true);
+}
+__device__ __forceinline__ unsigned aw_pack_root(const float (&r)[4], float& scale)
+{
+    const float big = aw_wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
+    const bool held = big >= AW_SMALLEST;
+    const float inv = held ? 1.0f / big : 0.0f;
+    scale = held ? big : 0.0f;
+    unsigned code = 0;
+    for (int k = 0; k < 4; k++) {
+        const unsigned bits = __float_as_uint(r[k] * inv);
+        const int c = (int)((bits + 0x3FFFFu + ((bits >> 19) & 1u)) >> 19) - AW_LEVEL0;
+        code |= (held && r[k] > 0.0f ? (unsigned)min(max(c, 1), 255) : 0u) << (8 * k);
+    }
+    return code;
+}
+
+// ---- the step ----
+template <int BITS, int PE, int GE>
+__device__ __forceinline__ void aw_update(const AwTensor& T, const AwState& S, const void* g_base, long i, int lane, const AwScal& s, float k, float keep)
+{
+    float p[4], g[4], m[4], v[4], root[4];
+    const long j = T.start + i;
+    aw_load<PE>(T.p, i, T.n, p);
+    aw_load<GE>(g_base, i, T.n, g);
+    if constexpr (BITS == 32) {
+        aw_load<0>((float*)S.m + T.start, i, T.n, m);
+        aw_load<0>((float*)S.v + T.start, i, T.n, v);
+    } else {
+        aw_mean_of(((const unsigned*)S.m)[j / 4], S.ms[j / AW_BLOCK], m);
+        aw_root_of(((const unsigned*)S.v)[j / 4], S.vs[j / AW_BLOCK], v);
+        for (int q = 0; q < 4; q++) v[q] = v[q] * v[q];
+    }
+    for (int q = 0; q < 4; q++) {
+        g[q] = g[q] * k;
+        m[q] = m[q] * s.b1 + g[q] * s.omb1;
+        v[q] = v[q] * s.b2 + g[q] * g[q] * s.omb2;
+        root[q] = sqrtf(v[q]);
+        p[q] = p[q] * keep - (m[q] / (root[q] * s.c1 + s.eps)) * s.c2;
+    }
+    aw_store<PE>(T.p, i, T.n, p);
+    if constexpr (BITS == 32) {
+        aw_store<0>((float*)S.m + T.start, i, T.n, m);
+        aw_store<0>((float*)S.v + T.start, i, T.n, v);
+    } else {
+        float ms, vs;
+        ((unsigned*)S.m)[j / 4] = aw_pack_mean(m, ms);
+        ((unsigned*)S.v)[j / 4] = aw_pack_root(root, vs);
+        if (lane == 0) {
+            S.ms[j / AW_BLOCK] = ms;
+            S.vs[j / AW_BLOCK] = vs;
+        }
+    }
+}
+
+template <int BITS>
+__global__ __launch_bounds__(256) void k_adamw(const AwTensor* __restrict__ tensors, const AwChunk* __restrict__ chunks, int base, AwState S,
+                                               AwGrads grads, AwScal s, const double* __restrict__ scal, const float* __restrict__ clip)
+{
+    const AwChunk ch = chunks[blockIdx.x];
+    const AwTensor T = tensors[ch.tensor];
+    const void* g = grads.g[ch.tensor - base];
+    if (!g) return;
+    const float k = clip ? clip[1] : 1.0f;
+    if (k != k) return;                                    // the gradients' norm is not finite: the step is skipped
+    if (scal) {
+        s.lr = scal[0];
+        s.c1 = (float)scal[1];
+        s.c2 = (float)scal[2];
+    }
+    const float keep = (float)(1.0 - s.lr * (double)T.decay);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int r = 0; r < AW_CHUNK / (4 * AW_BLOCK); r++) {
+        const long b0 = (long)ch.chunk * AW_CHUNK + (long)(r * 4 + wave) * AW_BLOCK;
+        if (b0 >= T.n) return;
+        const long i = b0 + lane * 4;
+        switch (T.ptype * 3 + T.gtype) {
+            case 0: aw_update<BITS, 0, 0>(T, S, g, i, lane, s, k, keep); break;
+            case 1: aw_update<BITS, 0, 1>(T, S, g, i, lane, s, k, keep); break;
+            case 2: aw_update<BITS, 0, 2>(T, S, g, i, lane, s, k, keep); break;
+            case 3: aw_update<BITS, 1, 0>(T, S, g, i, lane, s, k, keep); break;
+            case 4: aw_update<BITS, 1, 1>(T, S, g, i, lane, s, k, keep); break;
+            case 5: aw_update<BITS, 1, 2>(T, S, g, i, lane, s, k, keep); break;
+            case 6: aw_update<BITS, 2, 0>(T, S, g, i, lane, s, k, keep); break;
+            case 7: aw_update<BITS, 2, 1>(T, S, g, i, lane, s, k, keep); break;
+            default: aw_update<BITS, 2, 2>(T, S, g, i, lane, s, k, keep); break;
+        }
+    }
+}
+
+// ---- the norm: float64 partial sums per workgroup, then one workgroup adds them in order ----
+__device__ __forceinline__ double aw_block_sum(double x, double* lds)
+{
+    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    __syncthreads();
+    return x;
+}
+
+__global__ __launch_bounds__(256) void k_adamw_sumsq(const AwTensor* __restrict__ tensors, const AwChunk* __restrict__ chunks, int n_chunks, int base,
+                                                     AwGrads grads, double* __restrict__ partials, int add)
+{
+    __shared__ double lds[4];
+    double sum = 0.0;
+    for (int b = blockIdx.x; b < n_chunks; b += gridDim.x) {
+        const AwChunk ch = chunks[b];
+        const AwTensor& T = tensors[ch.tensor];
+        const void* g = grads.g[ch.tensor - base];
+        if (!g) continue;
+        for (int r = 0; r < AW_CHUNK / 1024; r++) {
+            const long i = (long)ch.chunk * AW_CHUNK + r * 1024 + threadIdx.x * 4;
+            float x[4];
+            if (T.gtype == 0) aw_load<0>(g, i, T.n, x);
+            else if (T.gtype == 1) aw_load<1>(g, i, T.n, x);
+            else aw_load<2>(g, i, T.n, x);
+            for (int q = 0; q < 4; q++) sum = fma((double)x[q], (double)x[q], sum);
+        }
+    }
+    sum = aw_block_sum(sum, lds);
+    if (threadIdx.x == 0) partials[blockIdx.x] = add ? partials[blockIdx.x] + sum : sum;
+}
+
+// out[0] = norm, out[1] = the coefficient min(1, max_norm / norm); NaN where the norm is not finite
+__global__ __launch_bounds__(256) void k_adamw_norm(const double* __restrict__ partials, int n, double max_norm, float* __restrict__ out)
+{
+    __shared__ double lds[4];
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) sum += partials[i];
+    sum = aw_block_sum(sum, lds);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(sum);
+        out[0] = (float)norm;
+        out[1] = !(norm <= (double)INFINITY) || norm == (double)INFINITY ? NAN : norm > max_norm ? (float)(max_norm / norm) : 1.0f;
+    }
+}
+
+// ---- 8-bit moments from and to float32 arrays of the same layout ----
+__global__ __launch_bounds__(256) void k_adamw_pack(const AwTensor* __restrict__ tensors, const AwChunk* __restrict__ chunks, AwState S,
+                                                    const float* __restrict__ m_in, const float* __restrict__ v_in)
+{
+    const AwChunk ch = chunks[blockIdx.x];
+    const AwTensor T = tensors[ch.tensor];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int r = 0; r < AW_CHUNK / (4 * AW_BLOCK); r++) {
+        const long b0 = (long)ch.chunk * AW_CHUNK + (long)(r * 4 + wave) * AW_BLOCK;
+        if (b0 >= T.n) return;
+        const long i = b0 + lane * 4, j = T.start + i;
+        float m[4], v[4], ms, vs;
+        aw_load<0>(m_in + T.start, i, T.n, m);
+        aw_load<0>(v_in + T.start, i, T.n, v);
+        for (int q = 0; q < 4; q++) v[q] = sqrtf(v[q]);
+        ((unsigned*)S.m)[j / 4] = aw_pack_mean(m, ms);
+        ((unsigned*)S.v)[j / 4] = aw_pack_root(v, vs);
+        if (lane == 0) {
+            S.ms[j / AW_BLOCK] = ms;
+            S.vs[j / AW_BLOCK] = vs;
+        }
+    }
+}
+
+// (the codes between a tensor's end and the next one's start are 0)
+__global__ __launch_bounds__(256) void k_adamw_unpack(AwState S, float* __restrict__ m_out, float* __restrict__ v_out, long quads)
+{
+    for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < quads; q += (long)gridDim.x * 256) {
+        float m[4], v[4];
+        aw_mean_of(((const unsigned*)S.m)[q], S.ms[q / (AW_BLOCK / 4)], m);
+        aw_root_of(((const unsigned*)S.v)[q], S.vs[q / (AW_BLOCK / 4)], v);
+        ((float4*)m_out)[q] = make_float4(m[0], m[1], m[2], m[3]);
+        ((float4*)v_out)[q] = make_float4(v[0] * v[0], v[1] * v[1], v[2] * v[2], v[3] * v[3]);
+    }
+}
+
+// ---- host ----
+static long aw_padded(int64_t n) { return (long)((n + AW_BLOCK - 1) / AW_BLOCK) * AW_BLOCK; }
+
+int64_t adamw_state_elems(int n, const int64_t* numels)
+{
+    int64_t total = 0;
+    for (int i = 0; i < n; i++) total += aw_padded(numels[i]);
+    return total;
+}
+
+static void aw_free(goai_adamw* o)
+{
+    if (!o) return;
+    (void)hipFree(o->d_tensors);
+    (void)hipFree(o->d_chunks);
+    (void)hipFree(o->d_partials);
+    delete o;
+}
+
+int adamw_check(int n, void* const* params, const int32_t* ptypes, const int32_t* gtypes, const int64_t* numels, const float* decays, int bits,
+                const void* m, const void* v, const float* ms, const float* vs)
+{
+    GOAI_REQUIRE(n >= 1, "adamw: no tensors");
+    GOAI_REQUIRE(params && ptypes && gtypes && numels && decays, "adamw: NULL table");
+    GOAI_REQUIRE(bits == 8 || bits == 32, "adamw: state_bits must be 8 or 32");
+    GOAI_REQUIRE(m && v && (bits == 32 || (ms && vs)), "adamw: NULL moments");
+    GOAI_REQUIRE((((uintptr_t)m | (uintptr_t)v) & 15) == 0 && (((uintptr_t)ms | (uintptr_t)vs) & 3) == 0, "adamw: moments must be 16-byte aligned");
+    int64_t chunks = 0;
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    for (int i = 0; i < n; i++) {
+        GOAI_REQUIRE(elem_ok(ptypes[i]) && elem_ok(gtypes[i]), "adamw: element type must be GOAI_ELEM_F32, GOAI_ELEM_BF16 or GOAI_ELEM_F16");
+        GOAI_REQUIRE(numels[i] >= 0 && numels[i] < (1LL << 40), "adamw: tensor size out of range");
+        GOAI_REQUIRE(isfinite(decays[i]) && decays[i] >= 0.0f, "adamw: weight decay must be finite and not negative");
+        chunks += (numels[i] + AW_CHUNK - 1) / AW_CHUNK;
+        if (!numels[i]) continue;
+        const uintptr_t at = (uintptr_t)params[i];
+        GOAI_REQUIRE(at != 0, "adamw: NULL parameter");
+        GOAI_REQUIRE(at % elem_bytes(ptypes[i]) == 0, "adamw: a parameter is not aligned to its element type");
+        spans.emplace_back(at, at + (uintptr_t)numels[i] * elem_bytes(ptypes[i]));
+    }
+    GOAI_REQUIRE(chunks < (1LL << 23), "adamw: too many elements");
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); i++) GOAI_REQUIRE(spans[i].first >= spans[i - 1].second, "adamw: parameters overlap in memory");
+    return GOAI_OK;
+}
+
+static int aw_build(goai_adamw* o, int n, void* const* params, const int32_t* ptypes, const int32_t* gtypes, const int64_t* numels,
+                    const float* decays)
+{
+    std::vector<AwChunk> chunks;
+    for (int i = 0; i < n; i++) {
+        o->tensors.push_back(AwTensor{ params[i], o->elems, (long)numels[i], decays[i], ptypes[i], gtypes[i] });
+        o->first.push_back((int)chunks.size());
+        for (int64_t k = 0; k * AW_CHUNK < numels[i]; k++) chunks.push_back(AwChunk{ i, (int)k });
+        o->elems += aw_padded(numels[i]);
+    }
+    o->first.push_back((int)chunks.size());
+    const size_t tb = o->tensors.size() * sizeof(AwTensor), cb = std::max<size_t>(chunks.size(), 1) * sizeof(AwChunk);
+    GOAI_HIP_CHECK(hipMalloc((void**)&o->d_tensors, tb));
+    GOAI_HIP_CHECK(hipMalloc((void**)&o->d_chunks, cb));
+    GOAI_HIP_CHECK(hipMalloc((void**)&o->d_partials, AW_NORM_BLOCKS * sizeof(double)));
+    GOAI_HIP_CHECK(hipMemcpy(o->d_tensors, o->tensors.data(), tb, hipMemcpyHostToDevice));
+    if (!chunks.empty()) GOAI_HIP_CHECK(hipMemcpy(o->d_chunks, chunks.data(), chunks.size() * sizeof(AwChunk), hipMemcpyHostToDevice));
+    return GOAI_OK;
+}
+
+int adamw_init(goai_ctx* c, int n, void* const* params, const int32_t* ptypes, const int32_t* gtypes, const int64_t* numels, const float* decays,
+               int bits, void* m, void* v, float* ms, float* vs, goai_adamw** out)
+{
+    goai_adamw* o = new goai_adamw();
+    o->device = c->device;
+    o->bits = bits;
+    o->state = AwState{ m, v, ms, vs };
+    int rc;
+    try {
+        rc = aw_build(o, n, params, ptypes, gtypes, numels, decays);
+    } catch (...) {
+        aw_free(o);
+        throw;
+    }
+    if (rc) {
+        aw_free(o);
+        return rc;
+    }
+    *out = o;
+    return GOAI_OK;
+}
+
+int adamw_destroy(goai_ctx* c, goai_adamw* o)
+{
+    GOAI_REQUIRE(o->device == c->device, "adamw: the optimiser lives on another GPU");
+    GOAI_HIP_CHECK(hipStreamSynchronize(c->stream));
+    aw_free(o);
+    return GOAI_OK;
+}
+
+// the launches of one pass over the tensors: AW_LAUNCH tensors at a time
+template <class F> static int aw_launches(const goai_adamw* o, const void* const* grads, F&& launch)
+{
+    const int n = (int)o->tensors.size();
+    for (int base = 0; base < n; base += AW_LAUNCH) {
+        const int end = std::min(n, base + AW_LAUNCH);
+        AwGrads g;
+        memset(&g, 0, sizeof(g));
+        for (int i = base; i < end; i++) g.g[i - base] = grads[i];
+        launch(base, o->d_chunks + o->first[base], o->first[end] - o->first[base], g);
+        GOAI_HIP_CHECK(hipGetLastError());
+    }
+    return GOAI_OK;
+}
+
+static int aw_check_grads(goai_ctx* c, const goai_adamw* o, const void* const* grads)
+{
+    GOAI_REQUIRE(o->device == c->device, "adamw: the optimiser lives on another GPU");
+    for (size_t i = 0; i < o->tensors.size(); i++)
+        GOAI_REQUIRE((uintptr_t)grads[i] % elem_bytes(o->tensors[i].gtype) == 0, "adamw: a gradient is not aligned to its element type");
+    return GOAI_OK;
+}
+
+int adamw_grad_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out)
+{
+    int rc = aw_check_grads(c, o, grads);
+    if (rc) return rc;
+    const int grid = std::max(1, std::min(AW_NORM_BLOCKS, o->first.back()));
+    rc = aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
+        k_adamw_sumsq<<<grid, 256, 0, c->stream>>>(o->d_tensors, chunks, n, base, g, o->d_partials, base != 0);
+    });
+    if (rc) return rc;
+    k_adamw_norm<<<1, 256, 0, c->stream>>>(o->d_partials, grid, max_norm, out);
+    GOAI_HIP_CHECK(hipGetLastError());
+    return GOAI_OK;
+}
+
+int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
+               const float* clip, const double* scalars)
+{
+    const int rc = aw_check_grads(c, o, grads);
+    if (rc) return rc;
+    if (!scalars) {
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        GOAI_HIP_CHECK(hipStreamIsCapturing(c->stream, &cap));
+        if (cap != hipStreamCaptureStatusNone) {
+            set_error("adamw: a captured step needs `scalars` on the device (lr and the bias corrections change from replay to replay)");
+            return GOAI_ERR_STATE;
+        }
+    }
+    AwScal s{ lr, (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
+              (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))), (float)(lr / (1.0 - pow(beta1, (double)t))) };
+    return aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
+        if (n == 0) return;
+        if (o->bits == 32) k_adamw<32><<<n, 256, 0, c->stream>>>(o->d_tensors, chunks, base, o->state, g, s, scalars, clip);
+        else k_adamw<8><<<n, 256, 0, c->stream>>>(o->d_tensors, chunks, base, o->state, g, s, scalars, clip);
+    });
+}
+
+int adamw_load_moments(goai_ctx* c, goai_adamw* o, const float* m, const float* v)
+{
+    GOAI_REQUIRE(o->device == c->device, "adamw: the optimiser lives on another GPU");
+    if (o->bits == 32) {
+        GOAI_HIP_CHECK(hipMemcpyAsync(o->state.m, m, o->elems * sizeof(float), hipMemcpyDeviceToDevice, c->stream));
+        GOAI_HIP_CHECK(hipMemcpyAsync(o->state.v, v, o->elems * sizeof(float), hipMemcpyDeviceToDevice, c->stream));
+        return GOAI_OK;
+    }
+    if (o->first.back()) k_adamw_pack<<<o->first.back(), 256, 0, c->stream>>>(o->d_tensors, o->d_chunks, o->state, m, v);
+    GOAI_HIP_CHECK(hipGetLastError());
+    return GOAI_OK;
+}
+
+int adamw_moments(goai_ctx* c, goai_adamw* o, float* m, float* v)
+{
+    GOAI_REQUIRE(o->device == c->device, "adamw: the optimiser lives on another GPU");
+    GOAI_REQUIRE((((uintptr_t)m | (uintptr_t)v) & 15) == 0, "adamw: moments must be 16-byte aligned");
+    if (o->bits == 32) {
+        GOAI_HIP_CHECK(hipMemcpyAsync(m, o->state.m, o->elems * sizeof(float), hipMemcpyDeviceToDevice, c->stream));
+        GOAI_HIP_CHECK(hipMemcpyAsync(v, o->state.v, o->elems * sizeof(float), hipMemcpyDeviceToDevice, c->stream));
+        return GOAI_OK;
+    }
+    const long quads = o->elems / 4;
+    if (quads) k_adamw_unpack<<<(unsigned)std::min<long>((quads + 255) / 256, 1 << 20), 256, 0, c->stream>>>(o->state, m, v, quads);
+    GOAI_HIP_CHECK(hipGetLastError());
+    return GOAI_OK;
+}
+
+}  // namespace goai

@@ -1,4 +1,5 @@
 // capi.hip -- extern "C" surface of libgoai_hip.so (declared in include/goai_hip.h).
+#include <exception>
 #include <new>
 #include <string>
 
@@ -474,6 +475,123 @@ int goai_profile_read(goai_ctx* ctx, double* conv_ms_total, int64_t* conv_launch
     for (hipEvent_t e : ctx->prof_events) (void)hipEventDestroy(e);
     ctx->prof_events.clear();
     return GOAI_OK;
+}
+
+// The argument checks come before the context's: they need no GPU.
+static int check_logprobs(const void* logits, int elem, int64_t stride, const uint8_t* valid, int64_t valid_stride, double temperature, int64_t rows,
+                          int cols)
+{
+    GOAI_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 30), "rows / cols out of range");
+    GOAI_REQUIRE(elem == GOAI_ELEM_F32 || elem == GOAI_ELEM_BF16 || elem == GOAI_ELEM_F16, "elem_type must be GOAI_ELEM_F32, GOAI_ELEM_BF16 or GOAI_ELEM_F16");
+    GOAI_REQUIRE(temperature >= 1e-4 && temperature <= 1e4, "temperature must be in 1e-4 .. 1e4");
+    GOAI_REQUIRE(rows == 0 || logits, "NULL logits");
+    GOAI_REQUIRE((uintptr_t)logits % (elem == GOAI_ELEM_F32 ? 4 : 2) == 0, "logits are not aligned to their element type");
+    GOAI_REQUIRE((stride >= cols || stride == 0) && (!valid || valid_stride >= cols || valid_stride == 0), "a row stride is smaller than the row");
+    return GOAI_OK;
+}
+
+int goai_action_logprobs(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid, int64_t valid_stride,
+                         const int32_t* actions, double temperature, int top, float* logp, float* entropy, float* lse, int32_t* top_actions,
+                         float* top_logp, int64_t rows, int cols)
+{
+    const int rc = check_logprobs(logits, elem_type, row_stride, valid, valid_stride, temperature, rows, cols);
+    if (rc) return rc;
+    GOAI_REQUIRE(top >= 0 && top <= GOAI_LOGPROBS_MAX_TOP, "top must be in 0 .. GOAI_LOGPROBS_MAX_TOP");
+    GOAI_REQUIRE(rows == 0 || top == 0 || (top_actions && top_logp), "top > 0 needs top_actions and top_logp");
+    GOAI_REQUIRE(rows == 0 || !logp || actions, "logp needs actions");
+    CTX_ENTER(ctx);
+    if (rows == 0) return GOAI_OK;
+    return launch_action_logprobs(logits, elem_type, row_stride, valid, valid_stride, actions, temperature, top, logp, entropy, lse, top_actions,
+                                  top_logp, rows, cols, ctx->stream);
+}
+
+int goai_action_logprobs_grad(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid, int64_t valid_stride,
+                              const int32_t* actions, double temperature, const float* lse, const float* entropy, const float* d_logp,
+                              const float* d_entropy, void* d_logits, int64_t d_stride, int64_t rows, int cols)
+{
+    const int rc = check_logprobs(logits, elem_type, row_stride, valid, valid_stride, temperature, rows, cols);
+    if (rc) return rc;
+    GOAI_REQUIRE(rows == 0 || (lse && d_logits), "NULL lse / d_logits");
+    GOAI_REQUIRE(rows == 0 || !d_logp || actions, "d_logp needs actions");
+    GOAI_REQUIRE(rows == 0 || !d_entropy || entropy, "d_entropy needs entropy");
+    GOAI_REQUIRE(d_stride >= cols, "d_stride is smaller than the row");
+    GOAI_REQUIRE((uintptr_t)d_logits % (elem_type == GOAI_ELEM_F32 ? 4 : 2) == 0, "d_logits is not aligned to its element type");
+    CTX_ENTER(ctx);
+    if (rows == 0) return GOAI_OK;
+    return launch_action_logprobs_grad(logits, elem_type, row_stride, valid, valid_stride, actions, temperature, lse, entropy, d_logp, d_entropy,
+                                       d_logits, d_stride, rows, cols, ctx->stream);
+}
+
+// host containers may throw; nothing leaves a C entry point
+#define GOAI_NO_THROW(...)                                                   \
+    try {                                                                    \
+        __VA_ARGS__;                                                         \
+    } catch (const std::exception& e) {                                      \
+        set_error(std::string("out of host memory: ") + e.what());           \
+        return GOAI_ERR_ARG;                                                 \
+    }
+
+int64_t goai_adamw_state_elems(int n_tensors, const int64_t* numels)
+{
+    GOAI_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || numels), "adamw: NULL table");
+    for (int i = 0; i < n_tensors; i++) GOAI_REQUIRE(numels[i] >= 0 && numels[i] < (1LL << 40), "adamw: tensor size out of range");
+    return adamw_state_elems(n_tensors, numels);
+}
+
+int goai_adamw_init(goai_ctx* ctx, int n_tensors, void* const* params, const int32_t* param_types, const int32_t* grad_types,
+                    const int64_t* numels, const float* weight_decays, int state_bits, void* exp_avg, void* exp_avg_sq, float* avg_scales,
+                    float* sq_scales, goai_adamw** out)
+{
+    GOAI_REQUIRE(out != nullptr, "out is NULL");
+    GOAI_NO_THROW({
+        const int rc = adamw_check(n_tensors, params, param_types, grad_types, numels, weight_decays, state_bits, exp_avg, exp_avg_sq, avg_scales,
+                                   sq_scales);
+        if (rc) return rc;
+        CTX_ENTER(ctx);
+        return adamw_init(ctx, n_tensors, params, param_types, grad_types, numels, weight_decays, state_bits, exp_avg, exp_avg_sq, avg_scales,
+                          sq_scales, out);
+    })
+}
+
+int goai_adamw_destroy(goai_ctx* ctx, goai_adamw* opt)
+{
+    if (!opt) return GOAI_OK;
+    CTX_ENTER(ctx);
+    return adamw_destroy(ctx, opt);
+}
+
+int goai_adamw_grad_norm(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, double max_norm, float* norm_and_coef)
+{
+    GOAI_REQUIRE(max_norm > 0.0, "adamw: max_norm must be positive");
+    GOAI_REQUIRE(opt && grads && norm_and_coef, "NULL argument");
+    CTX_ENTER(ctx);
+    return adamw_grad_norm(ctx, opt, grads, max_norm, norm_and_coef);
+}
+
+int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
+                    const float* norm_and_coef, const double* scalars)
+{
+    GOAI_REQUIRE(t >= 1, "adamw: the first step is t = 1");
+    GOAI_REQUIRE(lr >= 0.0 && lr <= 1e30, "adamw: lr must be finite and not negative");
+    GOAI_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw: betas must be in [0, 1)");
+    GOAI_REQUIRE(eps >= 1e-30 && eps <= 1e30, "adamw: eps must be in 1e-30 .. 1e30");
+    GOAI_REQUIRE(opt && grads, "NULL argument");
+    CTX_ENTER(ctx);
+    return adamw_step(ctx, opt, grads, t, lr, beta1, beta2, eps, norm_and_coef, scalars);
+}
+
+int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* exp_avg, const float* exp_avg_sq)
+{
+    GOAI_REQUIRE(opt && exp_avg && exp_avg_sq, "NULL argument");
+    CTX_ENTER(ctx);
+    return adamw_load_moments(ctx, opt, exp_avg, exp_avg_sq);
+}
+
+int goai_adamw_moments(goai_ctx* ctx, goai_adamw* opt, float* exp_avg, float* exp_avg_sq)
+{
+    GOAI_REQUIRE(opt && exp_avg && exp_avg_sq, "NULL argument");
+    CTX_ENTER(ctx);
+    return adamw_moments(ctx, opt, exp_avg, exp_avg_sq);
 }
 
 }  // extern "C"

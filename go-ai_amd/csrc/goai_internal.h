@@ -72,6 +72,27 @@ int comm_init(goai_ctx* c, const void* id128_host, int n_ranks, int rank, void**
 int comm_destroy(goai_ctx* c, void* comm);
 int gather_stats(goai_ctx* c, void* comm, double* extra_inout_host, int n_extra, int64_t* totals_host);
 
+// ---- log probabilities of actions (logprobs.hip) ----
+int launch_action_logprobs(const void* logits, int elem, int64_t stride, const uint8_t* valid, int64_t valid_stride, const int32_t* actions,
+                           double temperature, int top, float* logp, float* entropy, float* lse, int32_t* top_actions, float* top_logp,
+                           int64_t rows, int cols, hipStream_t st);
+int launch_action_logprobs_grad(const void* logits, int elem, int64_t stride, const uint8_t* valid, int64_t valid_stride,
+                                const int32_t* actions, double temperature, const float* lse, const float* entropy, const float* d_logp,
+                                const float* d_entropy, void* d_logits, int64_t d_stride, int64_t rows, int cols, hipStream_t st);
+
+// ---- AdamW over many tensors (adamw.hip) ----
+int64_t adamw_state_elems(int n, const int64_t* numels);
+int adamw_check(int n, void* const* params, const int32_t* ptypes, const int32_t* gtypes, const int64_t* numels, const float* decays, int bits,
+                const void* m, const void* v, const float* ms, const float* vs);
+int adamw_init(goai_ctx* c, int n, void* const* params, const int32_t* ptypes, const int32_t* gtypes, const int64_t* numels, const float* decays,
+               int bits, void* m, void* v, float* ms, float* vs, goai_adamw** out);
+int adamw_destroy(goai_ctx* c, goai_adamw* o);
+int adamw_grad_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out);
+int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
+               const float* clip, const double* scalars);
+int adamw_load_moments(goai_ctx* c, goai_adamw* o, const float* m, const float* v);
+int adamw_moments(goai_ctx* c, goai_adamw* o, float* m, float* v);
+
 // ---- search (mcts_host.hip) ----
 int mcts_init(goai_ctx* c, int n_games, int max_sims, int mode);
 int mcts_reset(goai_ctx* c, const uint8_t* roots);

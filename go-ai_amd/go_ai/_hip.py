@@ -74,6 +74,18 @@ _SIGNATURES = {
                         ctypes.POINTER(ctypes.c_float)],
     "goai_train_params": [c_void_p, ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64)],
     "goai_train_sync_inference": [c_void_p],
+    "goai_action_logprobs": [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_double, c_int, c_void_p, c_void_p, c_void_p,
+                             c_void_p, c_void_p, c_int64, c_int],
+    "goai_action_logprobs_grad": [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_double, c_void_p, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_int64, c_int64, c_int],
+    "goai_adamw_state_elems": [c_int, c_void_p],
+    "goai_adamw_init": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                        ctypes.POINTER(c_void_p)],
+    "goai_adamw_destroy": [c_void_p, c_void_p],
+    "goai_adamw_grad_norm": [c_void_p, c_void_p, c_void_p, c_double, c_void_p],
+    "goai_adamw_step": [c_void_p, c_void_p, c_void_p, c_int64, c_double, c_double, c_double, c_double, c_void_p, c_void_p],
+    "goai_adamw_load_moments": [c_void_p, c_void_p, c_void_p, c_void_p],
+    "goai_adamw_moments": [c_void_p, c_void_p, c_void_p, c_void_p],
     "goai_comm_unique_id": [c_void_p],
     "goai_comm_init": [c_void_p, c_void_p, c_int, c_int, ctypes.POINTER(c_void_p)],
     "goai_comm_destroy": [c_void_p, c_void_p],
@@ -84,7 +96,7 @@ _SIGNATURES = {
 
 for _name, _args in _SIGNATURES.items():
     _fn = getattr(lib, _name)          # AttributeError here = library older than this binding
-    _fn.restype = c_int
+    _fn.restype = c_int64 if _name == "goai_adamw_state_elems" else c_int
     _fn.argtypes = _args
 
 
@@ -103,3 +115,8 @@ def ptr(t):
         return None
     assert t.is_cuda and t.is_contiguous(), "libgoai_hip takes contiguous device tensors"
     return c_void_p(t.data_ptr())
+
+
+def dptr(t):
+    """Address of a device tensor (or None) whose strides the call is told."""
+    return None if t is None else t.data_ptr()

@@ -5,6 +5,7 @@ device tensors.  numpy inputs are accepted for convenience and copied to the GPU
 come back as torch device tensors (callers `.cpu().numpy()` them where the reference's
 surface promises numpy).
 """
+import collections
 import ctypes
 
 import numpy as np
@@ -23,6 +24,12 @@ def _dev_u8_states(states, device):
     if states.dtype != torch.uint8:
         states = (states != 0).to(torch.uint8)
     return states.to(device, non_blocking=True).contiguous()
+
+
+ELEM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # GOAI_ELEM_*
+
+# what Context.action_logprobs returns: float32 [rows] (logp None without actions) and [rows, top] (None for top = 0)
+ActionLogprobs = collections.namedtuple("ActionLogprobs", "logp entropy lse top_actions top_logp")
 
 
 class Context:
@@ -162,6 +169,99 @@ class Context:
         c_ptrs = (ctypes.c_void_p * n)(*[a.ctypes.data for a in arrays])
         c_numels = (ctypes.c_int64 * n)(*[a.size for a in arrays])
         _hip.check(_hip.lib.goai_load_weights(self._h, c_names, c_ptrs, c_numels, n))
+
+    # ---- log probabilities of actions, and their gradient ---------------------------------------
+    def _rows(self, x, what, rows=None, cols=None):
+        """A matrix on this GPU whose columns are next to each other (any row stride, 0 included), and its row stride."""
+        if not torch.is_tensor(x):
+            x = torch.as_tensor(np.asarray(x))
+        if x.dim() != 2 or (rows is not None and tuple(x.shape) != (rows, cols)):
+            raise ValueError(f"{what}: expected a matrix{'' if rows is None else f' of {rows} x {cols}'}, got shape {tuple(x.shape)}")
+        if x.device != self.device:
+            x = x.to(self.device)
+        rs, cs = x.stride()
+        n, m = x.shape
+        if (cs != 1 and m > 1) or (n > 1 and rs < m and rs != 0):
+            x = x.contiguous()
+            rs = m
+        return x, (rs if n > 1 else m)
+
+    def _logits_and_mask(self, logits, valid):
+        x, xs = self._rows(logits, "logits")
+        if x.dtype not in ELEM_TYPES:
+            if x.dtype != torch.float64:
+                raise ValueError(f"logits: float32, bfloat16 or float16 (float64 is rounded to float32), got {x.dtype}")
+            x = x.float().contiguous()
+            xs = x.shape[1]
+        v, vs = None, 0
+        if valid is not None:
+            v, vs = self._rows(valid, "valid", *x.shape)
+            if v.dtype is torch.bool:
+                v = v.view(torch.uint8)
+            elif v.dtype is not torch.uint8:
+                raise ValueError(f"valid: uint8 or bool, got {v.dtype}")
+        return x, xs, v, vs
+
+    def _per_row(self, x, rows, dtype, what):
+        if x is None:
+            return None
+        x = torch.as_tensor(x)
+        if x.dtype != dtype or x.device != self.device or not x.is_contiguous():
+            x = x.to(self.device, dtype=dtype).contiguous()
+        if x.numel() != rows:
+            raise ValueError(f"{what}: one number for each of the {rows} rows, got shape {tuple(x.shape)}")
+        return x
+
+    LOGPROBS_MAX_TOP = 64
+
+    def action_logprobs(self, logits, actions=None, valid=None, temperature=1.0, top=0):
+        """goai_action_logprobs: log probabilities of `actions` [rows] under softmax(logits / temperature) over the columns with
+        valid != 0 (uint8 / bool, None: all), the entropy, the log of the sum, and the `top` best columns with their log
+        probabilities.  logits [rows, columns]: float32, bfloat16 or float16 on the GPU (any row stride; an expanded row or mask
+        is read as it is); host arrays are copied.  actions < 0: none."""
+        self._bind()
+        x, xs, v, vs = self._logits_and_mask(logits, valid)
+        rows, cols = x.shape
+        a = self._per_row(actions, rows, torch.int32, "actions")
+        top = int(top)
+        if not 0 <= top <= self.LOGPROBS_MAX_TOP:
+            raise ValueError(f"top must be in 0 .. {self.LOGPROBS_MAX_TOP}")
+        out = torch.empty((3, rows), dtype=torch.float32, device=self.device)
+        logp, entropy, lse = out.unbind(0)
+        best = best_lp = None
+        if top:
+            best = torch.empty((rows, top), dtype=torch.int32, device=self.device)
+            best_lp = torch.empty((rows, top), dtype=torch.float32, device=self.device)
+        if a is None:
+            logp = None
+        if rows:
+            p = _hip.dptr
+            _hip.check(_hip.lib.goai_action_logprobs(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), temperature, top, p(logp),
+                                                     p(entropy), p(lse), p(best), p(best_lp), rows, cols))
+        return ActionLogprobs(logp, entropy, lse, best, best_lp)
+
+    def action_logprobs_grad(self, logits, actions, lse, entropy=None, d_logp=None, d_entropy=None, valid=None, temperature=1.0, out=None):
+        """goai_action_logprobs_grad: the gradient with respect to the logits (a dense matrix in their type) of a loss whose
+        gradients with respect to action_logprobs' logp and entropy are d_logp and d_entropy; lse and entropy are its outputs for
+        the same logits, valid and temperature.  out: a matrix to write into (the logits themselves, if nothing else reads them)."""
+        self._bind()
+        x, xs, v, vs = self._logits_and_mask(logits, valid)
+        rows, cols = x.shape
+        a = self._per_row(actions, rows, torch.int32, "actions")
+        l, e = self._per_row(lse, rows, torch.float32, "lse"), self._per_row(entropy, rows, torch.float32, "entropy")
+        g, h = self._per_row(d_logp, rows, torch.float32, "d_logp"), self._per_row(d_entropy, rows, torch.float32, "d_entropy")
+        if out is None:
+            out = torch.empty((rows, cols), dtype=x.dtype, device=self.device)
+        elif (out.dtype != x.dtype or tuple(out.shape) != (rows, cols) or out.device != self.device
+              or (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols)):
+            raise ValueError("out: a matrix of the logits' shape, type and device, its columns next to each other")
+        elif out.data_ptr() == x.data_ptr() and rows > 1 and out.stride(0) != xs:
+            raise ValueError("out: the logits themselves, or memory of its own")
+        if rows:
+            p = _hip.dptr
+            _hip.check(_hip.lib.goai_action_logprobs_grad(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), temperature, p(l), p(e), p(g),
+                                                          p(h), p(out), out.stride(0) if rows > 1 else cols, rows, cols))
+        return out
 
     # ---- result gather over ranks (goai_gather_stats) --------------------------------------
     @staticmethod

@@ -10,6 +10,8 @@ saved by the reference's train.py (utils.py:146-153) loads unchanged.
 import numpy as np
 import torch
 
+from .adamw import AdamW  # noqa: F401
+
 CHANNELS = 128
 LAYERS = 3
 

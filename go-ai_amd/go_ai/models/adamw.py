@@ -1,0 +1,214 @@
+"""AdamW over many tensors in one launch (goai_adamw_*), with the moments in 32 or in 8 bits."""
+import ctypes
+import math
+
+import torch
+
+BLOCK = 256          # elements that share one scale of an 8-bit moment
+
+
+def _ctypes_table(ctype, values):
+    return (ctype * max(len(values), 1))(*values)
+
+
+class AdamW:
+    """torch.optim.AdamW's update over a list of GPU tensors:
+
+        g = gradient * min(1, max_norm / |all gradients|)      (max_norm = 0: as it is)
+        m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+    params: contiguous tensors of one GPU (float32, bfloat16 or float16, in any mixture), or None / host tensors (what
+    RLNet.parameters() yields): then the optimiser belongs to the net that it is first handed to (RLNet.optimize,
+    RLNet.train_step), which gives it its parameters.  weight_decay and grad_dtype (None: each parameter's own type) are one value or
+    one per tensor.  state_bits = 8 holds the moments in a byte each, in blocks of 256 elements with a scale.
+
+    step(grads) takes the gradients as a list in the parameters' order (None: that tensor stays as it is).  With max_norm a norm
+    that is not finite leaves parameters and moments as they are; `norm` is the last step's norm (a GPU scalar).
+
+    A step can be captured into a graph: step(grads, captured=True) reads lr and the bias corrections from GPU memory when it
+    runs; call advance() before the capture's first replay and before every further one."""
+
+    def __init__(self, params=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=0.0,
+                 grad_dtype=None, ctx=None):
+        self.lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
+        self.weight_decay, self.state_bits, self.max_norm, self.grad_dtype = weight_decay, int(state_bits), float(max_norm), grad_dtype
+        if not (0.0 <= self.lr < math.inf and all(0.0 <= b < 1.0 for b in self.betas) and 1e-30 <= self.eps < math.inf):
+            raise ValueError("AdamW: lr >= 0, betas in [0, 1), eps >= 1e-30")
+        if self.state_bits not in (8, 32):
+            raise ValueError("AdamW: state_bits must be 8 or 32")
+        if not 0.0 <= self.max_norm:
+            raise ValueError("AdamW: max_norm must not be negative")
+        self.steps = 0
+        self.params = None
+        self._h = self._ctx = None
+        params = None if params is None else list(params)
+        if params and all(torch.is_tensor(p) and p.is_cuda for p in params):
+            self.bind(params, ctx)
+        elif params and any(torch.is_tensor(p) and p.is_cuda for p in params):
+            raise ValueError("AdamW: parameters on the GPU and on the host")
+
+    def zero_grad(self):
+        pass
+
+    # ---- parameters --------------------------------------------------------------------------
+    def bind(self, params, ctx=None):
+        """Take these GPU tensors as the parameters; fresh moments."""
+        from .. import _hip
+        from ..engine import ELEM_TYPES, Context
+        params = list(params)
+        n = len(params)
+        if not n:
+            raise ValueError("AdamW: no parameters")
+        device = params[0].device
+        for p in params:
+            if p.device != device or p.dtype not in ELEM_TYPES or not p.is_contiguous():
+                raise ValueError("AdamW: parameters are contiguous float32, bfloat16 or float16 tensors of one GPU, got "
+                                 f"{p.dtype} on {p.device}, strides {p.stride()}")
+
+        def each(x, what):
+            x = list(x) if isinstance(x, (list, tuple)) else [x] * n
+            if len(x) != n:
+                raise ValueError(f"AdamW: {n} parameters, {len(x)} values of {what}")
+            return x
+        decays = [float(d) for d in each(self.weight_decay, "weight_decay")]
+        gtypes = [p.dtype if g is None else g for p, g in zip(params, each(self.grad_dtype, "grad_dtype"))]
+        if any(g not in ELEM_TYPES for g in gtypes):
+            raise ValueError("AdamW: gradients are float32, bfloat16 or float16")
+        numels = _ctypes_table(ctypes.c_int64, [p.numel() for p in params])
+        elems = _hip.lib.goai_adamw_state_elems(n, numels)
+        state = torch.uint8 if self.state_bits == 8 else torch.float32
+        blocks = max(elems, 1) // BLOCK if self.state_bits == 8 else 0
+        m, v = [torch.zeros(elems, dtype=state, device=device) for _ in range(2)]
+        scales = torch.zeros((2, max(blocks, 1)), dtype=torch.float32, device=device)
+        self.close()
+        self._ctx = ctx if ctx is not None else Context(9, device.index)
+        self._ctx._bind()
+        h = ctypes.c_void_p()
+        eight = self.state_bits == 8
+        _hip.check(_hip.lib.goai_adamw_init(
+            self._ctx._h, n, _ctypes_table(ctypes.c_void_p, [p.data_ptr() for p in params]),
+            _ctypes_table(ctypes.c_int32, [ELEM_TYPES[p.dtype] for p in params]), _ctypes_table(ctypes.c_int32, [ELEM_TYPES[g] for g in gtypes]),
+            numels, _ctypes_table(ctypes.c_float, decays), self.state_bits, m.data_ptr() or scales.data_ptr(), v.data_ptr() or scales.data_ptr(),
+            scales[0].data_ptr() if eight else None, scales[1].data_ptr() if eight else None, ctypes.byref(h)))
+        self._h = h
+        self.params, self.device = params, device
+        self._gtypes, self._shapes = gtypes, [p.shape for p in params]
+        self._m, self._v, self._scales, self._elems = m, v, scales, elems
+        self._table = _ctypes_table(ctypes.c_void_p, [None] * n)
+        self._clip = torch.zeros(2, dtype=torch.float32, device=device)
+        self._scalars = None
+        self.offsets, at = [], 0
+        for p in params:
+            self.offsets.append(at)
+            at += -(-p.numel() // BLOCK) * BLOCK
+        self.steps = 0
+        return self
+
+    def close(self):
+        if self._h is not None and self._ctx is not None and not self._ctx.closed:
+            from .. import _hip
+            _hip.lib.goai_adamw_destroy(self._ctx._h, self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _bound(self):
+        if self._h is None:
+            raise RuntimeError("AdamW: no parameters yet: give it GPU tensors, or hand it to a net's train_step / optimize")
+        self._ctx._bind()
+
+    # ---- the step ----------------------------------------------------------------------------
+    def _grads(self, grads):
+        if len(grads) != len(self.params):
+            raise ValueError(f"AdamW: {len(self.params)} parameters, {len(grads)} gradients")
+        table, device = self._table, self.device
+        for i, (g, dtype, shape) in enumerate(zip(grads, self._gtypes, self._shapes)):
+            if g is None:
+                table[i] = None
+            elif g.dtype is dtype and g.shape == shape and g.device == device and g.is_contiguous():
+                table[i] = g.data_ptr()
+            else:
+                raise ValueError(f"AdamW: gradient {i} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, got {g.dtype} "
+                                 f"of shape {tuple(g.shape)} on {g.device}, strides {g.stride()}")
+        return table
+
+    def advance(self):
+        """The next step's number; writes lr and the bias corrections of that step where a captured step reads them."""
+        self._bound()
+        if self._scalars is None:
+            self._scalars = torch.zeros(3, dtype=torch.float64, device=self.device)
+        self.steps += 1
+        b1, b2 = self.betas
+        self._scalars.copy_(torch.tensor([self.lr, 1.0 / math.sqrt(1.0 - b2 ** self.steps), self.lr / (1.0 - b1 ** self.steps)],
+                                         dtype=torch.float64))
+
+    def step(self, grads, captured=False):
+        """One step on the current stream; the number of the step is `steps` + 1 (captured: see advance)."""
+        from .. import _hip
+        self._bound()
+        table = self._grads(grads)
+        if captured and self._scalars is None:
+            raise RuntimeError("AdamW: call advance() before a captured step")
+        clip = None
+        if self.max_norm:
+            clip = self._clip.data_ptr()
+            _hip.check(_hip.lib.goai_adamw_grad_norm(self._ctx._h, self._h, table, self.max_norm, clip))
+        t = self.steps if captured else self.steps + 1
+        _hip.check(_hip.lib.goai_adamw_step(self._ctx._h, self._h, table, max(t, 1), self.lr, self.betas[0], self.betas[1], self.eps, clip,
+                                            self._scalars.data_ptr() if captured else None))
+        self.steps = t
+
+    @property
+    def norm(self):
+        """The gradients' global norm at the last step with max_norm (before clipping): a GPU scalar."""
+        return self._clip[0]
+
+    # ---- moments -----------------------------------------------------------------------------
+    def moments(self):
+        """(exp_avg, exp_avg_sq) as flat float32 GPU tensors: tensor i's at [offsets[i] : offsets[i] + numel].  The optimiser's own
+        buffers for state_bits = 32, the values that the codes stand for (new tensors) for 8."""
+        self._bound()
+        if self.state_bits == 32:
+            return self._m, self._v
+        from .. import _hip
+        m, v = [torch.empty(self._elems, dtype=torch.float32, device=self.device) for _ in range(2)]
+        if self._elems:
+            _hip.check(_hip.lib.goai_adamw_moments(self._ctx._h, self._h, m.data_ptr(), v.data_ptr()))
+        return m, v
+
+    def _split(self, flat):
+        return [flat[a:a + p.numel()].view(p.shape) for a, p in zip(self.offsets, self.params)]
+
+    def load_moments(self, exp_avg, exp_avg_sq, steps):
+        """Continue from these moments (one float tensor per parameter) after `steps` steps; 8-bit moments are rounded to their codes."""
+        self._bound()
+        if len(exp_avg) != len(self.params) or len(exp_avg_sq) != len(self.params):
+            raise ValueError(f"AdamW: {len(self.params)} parameters, moments for {len(exp_avg)} and {len(exp_avg_sq)}")
+        if int(steps) < 0:
+            raise ValueError("AdamW: steps must not be negative")
+        for a, b, s in zip(exp_avg, exp_avg_sq, self._shapes):
+            if a.shape != s or b.shape != s:
+                raise ValueError(f"AdamW: a parameter of shape {tuple(s)}, moments of shapes {tuple(a.shape)} and {tuple(b.shape)}")
+        flat = (self._m, self._v)
+        if self.state_bits == 8:
+            flat = [torch.zeros(self._elems, dtype=torch.float32, device=self.device) for _ in range(2)]
+        for to, given in zip(flat, (exp_avg, exp_avg_sq)):
+            for dst, src in zip(self._split(to), given):
+                dst.copy_(src)
+        if self.state_bits == 8 and self._elems:
+            from .. import _hip
+            _hip.check(_hip.lib.goai_adamw_load_moments(self._ctx._h, self._h, flat[0].data_ptr(), flat[1].data_ptr()))
+        self.steps = int(steps)
+
+    def state_dict(self):
+        """steps and the moments as float32 host tensors in the parameters' order."""
+        m, v = self.moments()
+        return {"steps": self.steps, "exp_avg": [x.cpu().clone() for x in self._split(m)], "exp_avg_sq": [x.cpu().clone() for x in self._split(v)]}
+
+    def load_state_dict(self, state):
+        self.load_moments(state["exp_avg"], state["exp_avg_sq"], state["steps"])

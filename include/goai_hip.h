@@ -385,6 +385,86 @@ int goai_train_params(goai_ctx* ctx, float** params_device, int64_t* numel);
 int goai_train_sync_inference(goai_ctx* ctx);
 
 /* ---------------------------------------------------------------------------------------
+ * Log probabilities of actions, and their gradient: what a policy gives the moves that were played, how undecided it is, and
+ * what it would rather have played -- for scoring recorded games, analysis, and losses of the policy-gradient kind (the reference
+ * has the cross entropy of one greedy target alone, /root/reference/go_ai/models/__init__.py:175-184; goai_train_step keeps it).
+ * Any number of columns: the S*S + 1 actions of a board, or any other choice.
+ * ------------------------------------------------------------------------------------- */
+#define GOAI_ELEM_F32 0   /* element types of caller-owned arrays */
+#define GOAI_ELEM_BF16 1
+#define GOAI_ELEM_F16 2
+#define GOAI_LOGPROBS_MAX_TOP 64
+
+/* For each of `rows` rows of `cols` logits (row i at logits + i * row_stride elements; row_stride >= cols, or 0: one row for all)
+ * at `temperature` (1e-4 .. 1e4): over the allowed columns -- valid != 0 (uint8, row stride valid_stride, 0: one mask for
+ * all rows; NULL: all) and logit > -inf -- of softmax(logits / temperature),
+ *   logp[i]     the log probability of actions[i]: -inf where that column is not allowed, 0 where actions[i] < 0 (no action),
+ *               NaN where actions[i] >= cols;
+ *   entropy[i]  in nats;   lse[i]  log of the sum of exp(logit / temperature);
+ *   top_actions[i][top], top_logp[i][top]  the best columns, best first, of equal logits the lower one, and their log
+ *               probabilities; -1 and -inf behind the last allowed column.  0 <= top <= GOAI_LOGPROBS_MAX_TOP.
+ * A row without allowed columns has entropy 0 and lse = logp = -inf.  What stands in columns that are not allowed is never
+ * used (NaN and infinities included).  A NaN or +inf among the allowed logits makes the row's numbers NaN (a NaN is never
+ * listed).  logp (with actions), entropy, lse may be NULL.  Sums are float32 whatever the logits' type. */
+int goai_action_logprobs(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid,
+                         int64_t valid_stride, const int32_t* actions, double temperature, int top, float* logp, float* entropy,
+                         float* lse, int32_t* top_actions, float* top_logp, int64_t rows, int cols);
+
+/* The gradient with respect to the logits of a loss whose gradients with respect to logp and entropy are d_logp and
+ * d_entropy (float32 [rows]; either may be NULL: 0):
+ *   d_logits[i][j] = (d_logp (delta(actions[i], j) - p_j) - d_entropy p_j (log p_j + entropy)) / temperature
+ * on allowed columns, 0 on the others; in the logits' type.  lse and entropy (needed with d_entropy) are goai_action_logprobs'
+ * outputs for the same logits, mask and temperature.  A row whose actions[i] < 0 has no d_logp term; actions[i] >= cols
+ * makes the row NaN.  d_logits may be the logits themselves when d_stride == row_stride; otherwise they must not overlap. */
+int goai_action_logprobs_grad(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid,
+                              int64_t valid_stride, const int32_t* actions, double temperature, const float* lse,
+                              const float* entropy, const float* d_logp, const float* d_entropy, void* d_logits, int64_t d_stride,
+                              int64_t rows, int cols);
+
+/* ---------------------------------------------------------------------------------------
+ * AdamW over many tensors at once (goai_train_step's Adam folds the weight decay into the gradient,
+ * /root/reference/train.py:52; here it shrinks the parameter itself), with the moments in 32 or in 8 bits and clipping by the
+ * gradients' global norm.
+ * ------------------------------------------------------------------------------------- */
+typedef struct goai_adamw goai_adamw;
+
+/* Elements of the moments' flat arrays: every tensor starts at a multiple of 256 elements, in the order given. */
+int64_t goai_adamw_state_elems(int n_tensors, const int64_t* numels);
+
+/* Tables (HOST) over the tensors: parameters (DEVICE, contiguous, not overlapping), element types of parameters and
+ * gradients (GOAI_ELEM_*), sizes, weight decays.  The caller owns parameters and moments; they must outlive `out`.
+ *   state_bits 32: exp_avg, exp_avg_sq float32 [elems];  avg_scales, sq_scales NULL
+ *   state_bits 8:  exp_avg, exp_avg_sq uint8 [elems], avg_scales, sq_scales float32 [elems / 256]: codes and scales of the first
+ *                  moment (e4m3) and of the second one's root, in blocks of 256 elements
+ * The moments start as the caller left them (all zeros: a fresh optimiser); 16-byte aligned.  elems as above. */
+int goai_adamw_init(goai_ctx* ctx, int n_tensors, void* const* params, const int32_t* param_types, const int32_t* grad_types,
+                    const int64_t* numels, const float* weight_decays, int state_bits, void* exp_avg, void* exp_avg_sq,
+                    float* avg_scales, float* sq_scales, goai_adamw** out);
+/* Synchronises the stream. */
+int goai_adamw_destroy(goai_ctx* ctx, goai_adamw* opt);
+
+/* The 2-norm over all gradients (grads: HOST table of DEVICE pointers; NULL: the tensor has none) and the clipping coefficient
+ * min(1, max_norm / norm) into norm_and_coef[2] (DEVICE); the coefficient is NaN when the norm is not finite.  Summed in
+ * float64 in a fixed order.  max_norm = INFINITY: the norm alone. */
+int goai_adamw_grad_norm(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, double max_norm, float* norm_and_coef);
+
+/* Step number t (from 1): with g the gradient times the coefficient of norm_and_coef (DEVICE, may be NULL: 1),
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in float32, rounded to the parameter's type and the moments' bits at the end.  A NaN coefficient leaves everything as it is,
+ * a tensor without a gradient stays as it is.  A gradient whose
+ * square is beyond float32 (|g| >= 2^64 after clipping) gives its element -- with 8 bits every element of its block that is not
+ * zero -- an infinite second moment, which stays; one that is not finite spoils its element or block likewise.  scalars: NULL, or DEVICE double[3] = { lr, 1 / sqrt(1 - beta2^t), lr / (1 - beta1^t) },
+ * read when the step runs, in place of lr and t: a step that is captured into a graph needs it (GOAI_ERR_STATE without), and the
+ * graph's owner updates it between replays.  Two calls on the same optimiser must not run at the same time. */
+int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, int64_t t, double lr, double beta1, double beta2,
+                    double eps, const float* norm_and_coef, const double* scalars);
+
+/* Moments from / to float32 arrays [elems] of the flat layout (16-byte aligned), rounding to / reading the 8-bit codes. */
+int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* exp_avg, const float* exp_avg_sq);
+int goai_adamw_moments(goai_ctx* ctx, goai_adamw* opt, float* exp_avg, float* exp_avg_sq);
+
+/* ---------------------------------------------------------------------------------------
  * The one collective of the path: the end-of-run sums over ranks that the reference makes with
  * comm.allreduce(..., op=MPI.SUM) (/root/reference/go_ai/utils.py:201-204: seconds per game, win
  * rates, steps).  Games are sharded over GPUs and the search never communicates; this is an RCCL

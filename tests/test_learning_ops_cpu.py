@@ -1,0 +1,108 @@
+"""What the learning operators' entry points refuse: the argument checks come before the context's and need no GPU."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from go_ai import _hip
+
+P = ctypes.c_void_p
+lib = _hip.lib
+
+
+def err():
+    return lib.goai_last_error().decode()
+
+
+def logprobs(**k):
+    a = dict(logits=64, elem=0, stride=82, valid=None, vstride=0, actions=64, t=1.0, top=0, logp=64, ent=64, lse=64, ta=None, tl=None, rows=4, cols=82)
+    a.update(k)
+    return lib.goai_action_logprobs(None, a["logits"], a["elem"], a["stride"], a["valid"], a["vstride"], a["actions"], a["t"], a["top"], a["logp"],
+                                    a["ent"], a["lse"], a["ta"], a["tl"], a["rows"], a["cols"])
+
+
+@pytest.mark.parametrize("bad,message", [
+    (dict(), "ctx is NULL"), (dict(rows=-1), "rows"), (dict(cols=0), "cols"), (dict(cols=(1 << 30) + 1), "cols"), (dict(elem=3), "elem_type"),
+    (dict(elem=-1), "elem_type"), (dict(t=0.0), "temperature"), (dict(t=math.nan), "temperature"), (dict(t=math.inf), "temperature"),
+    (dict(t=-1.0), "temperature"), (dict(logits=None), "logits"), (dict(logits=66), "aligned"), (dict(logits=65, elem=1), "aligned"),
+    (dict(stride=81), "stride"), (dict(stride=-82), "stride"), (dict(valid=64, vstride=5), "stride"), (dict(top=65), "top"), (dict(top=-1), "top"),
+    (dict(top=3), "top_actions"), (dict(top=3, ta=64), "top_logp"), (dict(actions=None), "actions"), (dict(rows=0, logits=None), "ctx is NULL"),
+])
+def test_logprobs(bad, message):
+    assert logprobs(**bad) == -1 and message in err()
+
+
+def grad(**k):
+    a = dict(logits=64, elem=0, stride=82, actions=64, t=1.0, lse=64, ent=64, g=64, h=64, d=64, ds=82, rows=4, cols=82)
+    a.update(k)
+    return lib.goai_action_logprobs_grad(None, a["logits"], a["elem"], a["stride"], None, 0, a["actions"], a["t"], a["lse"], a["ent"], a["g"], a["h"],
+                                         a["d"], a["ds"], a["rows"], a["cols"])
+
+
+@pytest.mark.parametrize("bad,message", [
+    (dict(), "ctx is NULL"), (dict(lse=None), "lse"), (dict(d=None), "d_logits"), (dict(actions=None), "actions"), (dict(ent=None), "entropy"),
+    (dict(ds=81), "d_stride"), (dict(ds=0), "d_stride"), (dict(d=66), "aligned"), (dict(t=0.0), "temperature"), (dict(logits=None), "logits"),
+    (dict(ent=None, h=None), "ctx is NULL"), (dict(actions=None, g=None), "ctx is NULL"),
+])
+def test_gradient(bad, message):
+    assert grad(**bad) == -1 and message in err()
+
+
+def init(**k):
+    a = dict(n=2, params=[256, 1024], pt=[0, 1], gt=[0, 1], numels=[10, 300], decays=[0.0, 0.1], bits=8, m=64, v=64, ms=64, vs=64)
+    a.update(k)
+    t = lambda c, x: None if x is None else (c * max(len(x), 1))(*x)  # noqa: E731
+    out = P()
+    return lib.goai_adamw_init(None, a["n"], t(P, a["params"]), t(ctypes.c_int32, a["pt"]), t(ctypes.c_int32, a["gt"]), t(ctypes.c_int64, a["numels"]),
+                               t(ctypes.c_float, a["decays"]), a["bits"], a["m"], a["v"], a["ms"], a["vs"], ctypes.byref(out))
+
+
+@pytest.mark.parametrize("bad,message", [
+    (dict(), "ctx is NULL"), (dict(n=0), "no tensors"), (dict(params=None), "NULL table"), (dict(numels=None), "NULL table"),
+    (dict(decays=None), "NULL table"), (dict(pt=None), "NULL table"), (dict(gt=None), "NULL table"), (dict(bits=16), "state_bits"),
+    (dict(m=None), "moments"), (dict(v=None), "moments"), (dict(ms=None), "moments"), (dict(m=72), "16-byte"), (dict(pt=[0, 3]), "element type"),
+    (dict(gt=[-1, 0]), "element type"), (dict(numels=[-1, 3]), "size"), (dict(decays=[0.0, -1.0]), "decay"), (dict(decays=[math.nan, 0.0]), "decay"),
+    (dict(params=[None, 1024]), "NULL parameter"), (dict(params=[258, 1024]), "aligned"), (dict(params=[256, 1025]), "aligned"),
+    (dict(params=[1020, 1024]), "overlap"), (dict(params=[256, 256]), "overlap"), (dict(params=[None, 1024], numels=[0, 300]), "ctx is NULL"),
+    (dict(bits=32, ms=None, vs=None), "ctx is NULL"), (dict(numels=[1 << 39, 300], params=[1 << 41, 1024]), "too many"),
+])
+def test_adamw_init(bad, message):
+    assert init(**bad) == -1 and message in err()
+
+
+def test_adamw_state_elems():
+    n = (ctypes.c_int64 * 5)(0, 1, 256, 257, 1 << 33)
+    assert lib.goai_adamw_state_elems(5, n) == 256 + 256 + 512 + (1 << 33)
+    assert lib.goai_adamw_state_elems(0, None) == 0
+    assert lib.goai_adamw_state_elems(1, None) == -1
+    assert lib.goai_adamw_state_elems(1, (ctypes.c_int64 * 1)(-5)) == -1
+
+
+def test_adamw_calls():
+    table = (P * 1)(64)
+    step = lambda t=1, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, opt=64, g=table: lib.goai_adamw_step(None, opt, g, t, lr, b1, b2, eps, None, None)  # noqa: E731
+    for bad, message in ((dict(t=0), "t = 1"), (dict(lr=-1.0), "lr"), (dict(lr=math.nan), "lr"), (dict(lr=math.inf), "lr"), (dict(b1=1.0), "betas"),
+                         (dict(b2=-0.1), "betas"), (dict(b2=math.nan), "betas"), (dict(eps=0.0), "eps"), (dict(eps=math.nan), "eps"),
+                         (dict(opt=None), "NULL"), (dict(g=None), "NULL"), (dict(), "ctx is NULL")):
+        assert step(**bad) == -1 and message in err(), bad
+    norm = lambda m=1.0, opt=64, g=table, out=64: lib.goai_adamw_grad_norm(None, opt, g, m, out)  # noqa: E731
+    for bad, message in ((dict(m=0.0), "max_norm"), (dict(m=-1.0), "max_norm"), (dict(m=math.nan), "max_norm"), (dict(opt=None), "NULL"),
+                         (dict(g=None), "NULL"), (dict(out=None), "NULL"), (dict(), "ctx is NULL")):
+        assert norm(**bad) == -1 and message in err(), bad
+    assert lib.goai_adamw_load_moments(None, 64, None, 64) == -1 and lib.goai_adamw_moments(None, 64, 64, None) == -1
+    assert lib.goai_adamw_destroy(None, None) == 0
+
+
+def test_adamw_without_a_gpu_is_only_numbers():
+    """Host parameters (RLNet.parameters) or none: the optimiser waits for the net it is handed to."""
+    import torch
+    from go_ai.models import AdamW
+    for params in (None, [], [torch.zeros(3), torch.zeros(2, 2)]):
+        opt = AdamW(params, lr=0.1, weight_decay=0.0)
+        assert opt.params is None and opt.lr == 0.1
+        with pytest.raises(RuntimeError, match="no parameters yet"):
+            opt.step([])
+    for bad in (dict(lr=-1), dict(betas=(0.9, 1.0)), dict(eps=0), dict(state_bits=4), dict(max_norm=-1)):
+        with pytest.raises(ValueError):
+            AdamW(None, **bad)
