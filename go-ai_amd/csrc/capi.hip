@@ -481,7 +481,7 @@ int goai_profile_read(goai_ctx* ctx, double* conv_ms_total, int64_t* conv_launch
 static int check_logprobs(const void* logits, int elem, int64_t stride, const uint8_t* valid, int64_t valid_stride, double temperature, int64_t rows,
                           int cols)
 {
-    GOAI_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 30), "rows / cols out of range");
+    GOAI_REQUIRE(rows >= 0 && rows <= (1LL << 40) && cols >= 1 && cols <= (1 << 30), "rows / cols out of range");
     GOAI_REQUIRE(elem == GOAI_ELEM_F32 || elem == GOAI_ELEM_BF16 || elem == GOAI_ELEM_F16, "elem_type must be GOAI_ELEM_F32, GOAI_ELEM_BF16 or GOAI_ELEM_F16");
     GOAI_REQUIRE(temperature >= 1e-4 && temperature <= 1e4, "temperature must be in 1e-4 .. 1e4");
     GOAI_REQUIRE(rows == 0 || logits, "NULL logits");
@@ -492,17 +492,27 @@ static int check_logprobs(const void* logits, int elem, int64_t stride, const ui
 
 int goai_action_logprobs(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid, int64_t valid_stride,
                          const int32_t* actions, double temperature, int top, float* logp, float* entropy, float* lse, int32_t* top_actions,
-                         float* top_logp, int64_t rows, int cols)
+                         float* top_logp, int64_t rows, int cols, void* workspace, int64_t workspace_bytes)
 {
     const int rc = check_logprobs(logits, elem_type, row_stride, valid, valid_stride, temperature, rows, cols);
     if (rc) return rc;
     GOAI_REQUIRE(top >= 0 && top <= GOAI_LOGPROBS_MAX_TOP, "top must be in 0 .. GOAI_LOGPROBS_MAX_TOP");
     GOAI_REQUIRE(rows == 0 || top == 0 || (top_actions && top_logp), "top > 0 needs top_actions and top_logp");
     GOAI_REQUIRE(rows == 0 || !logp || actions, "logp needs actions");
+    const int64_t need = action_logprobs_workspace(rows, cols, top);
+    GOAI_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                 "the workspace is too small (goai_action_logprobs_workspace) or not 16-byte aligned");
     CTX_ENTER(ctx);
     if (rows == 0) return GOAI_OK;
     return launch_action_logprobs(logits, elem_type, row_stride, valid, valid_stride, actions, temperature, top, logp, entropy, lse, top_actions,
-                                  top_logp, rows, cols, ctx->stream);
+                                  top_logp, rows, cols, workspace, ctx->stream);
+}
+
+int64_t goai_action_logprobs_workspace(int64_t rows, int cols, int top)
+{
+    GOAI_REQUIRE(rows >= 0 && rows <= (1LL << 40) && cols >= 1 && cols <= (1 << 30), "rows / cols out of range");
+    GOAI_REQUIRE(top >= 0 && top <= GOAI_LOGPROBS_MAX_TOP, "top must be in 0 .. GOAI_LOGPROBS_MAX_TOP");
+    return action_logprobs_workspace(rows, cols, top);
 }
 
 int goai_action_logprobs_grad(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid, int64_t valid_stride,

@@ -28,6 +28,26 @@ template <int E> __device__ __forceinline__ typename Elem<E>::raw elem_from_floa
     else return __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
+// N neighbouring elements by wide accesses; the address is aligned to the element type only (gfx950 takes that in global memory)
+template <int E, int N> struct ElemVec {
+    using raw = typename Elem<E>::raw;
+    raw a[N];
+};
+template <int E, int N> __device__ __forceinline__ void elem_load(const typename Elem<E>::raw* p, float (&out)[N])
+{
+    ElemVec<E, N> v;
+    __builtin_memcpy(&v, p, sizeof(v));
+#pragma unroll
+    for (int k = 0; k < N; k++) out[k] = elem_to_float<E>(v.a[k]);
+}
+template <int E, int N> __device__ __forceinline__ void elem_store(typename Elem<E>::raw* p, const float (&x)[N])
+{
+    ElemVec<E, N> v;
+#pragma unroll
+    for (int k = 0; k < N; k++) v.a[k] = elem_from_float<E>(x[k]);
+    __builtin_memcpy(p, &v, sizeof(v));
+}
+
 inline int elem_bytes(int e) { return e == 0 ? 4 : 2; }
 inline bool elem_ok(int e) { return e >= 0 && e <= 2; }
 

@@ -75,7 +75,8 @@ int gather_stats(goai_ctx* c, void* comm, double* extra_inout_host, int n_extra,
 // ---- log probabilities of actions (logprobs.hip) ----
 int launch_action_logprobs(const void* logits, int elem, int64_t stride, const uint8_t* valid, int64_t valid_stride, const int32_t* actions,
                            double temperature, int top, float* logp, float* entropy, float* lse, int32_t* top_actions, float* top_logp,
-                           int64_t rows, int cols, hipStream_t st);
+                           int64_t rows, int cols, void* workspace, hipStream_t st);
+int64_t action_logprobs_workspace(int64_t rows, int cols, int top);
 int launch_action_logprobs_grad(const void* logits, int elem, int64_t stride, const uint8_t* valid, int64_t valid_stride,
                                 const int32_t* actions, double temperature, const float* lse, const float* entropy, const float* d_logp,
                                 const float* d_entropy, void* d_logits, int64_t d_stride, int64_t rows, int cols, hipStream_t st);

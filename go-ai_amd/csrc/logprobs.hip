@@ -50,33 +50,137 @@ __device__ __forceinline__ void lp_raise(LpStat& s, float m, LpFactor c)     // 
     s.m = m;
 }
 
+// ---- cross-lane helpers: lanes in rows of 16 by DPP, beyond that by shuffles ----
+template <int CTRL> __device__ __forceinline__ int lp_dpp(int x) { return __builtin_amdgcn_mov_dpp(x, CTRL, 0xf, 0xf, true); }
+template <int CTRL> __device__ __forceinline__ float lp_dpp(float x) { return __int_as_float(lp_dpp<CTRL>(__float_as_int(x))); }
+constexpr int ROR = 0x120, MIRROR = 0x140, HALF_MIRROR = 0x141, XOR1 = 0xb1, XOR2 = 0x4e, XOR3 = 0x1b;
+
+// over groups of L = 16 or 64 lanes, the result in all of them
+template <int L> __device__ __forceinline__ float lp_max(float x)
+{
+    x = fmaxf(x, lp_dpp<ROR + 8>(x));
+    x = fmaxf(x, lp_dpp<ROR + 4>(x));
+    x = fmaxf(x, lp_dpp<ROR + 2>(x));
+    x = fmaxf(x, lp_dpp<ROR + 1>(x));
+    if constexpr (L == 64) {
+        x = fmaxf(x, __shfl_xor(x, 16));
+        x = fmaxf(x, __shfl_xor(x, 32));
+    }
+    return x;
+}
+template <int L> __device__ __forceinline__ float lp_sum(float x)
+{
+    x += lp_dpp<ROR + 8>(x);
+    x += lp_dpp<ROR + 4>(x);
+    x += lp_dpp<ROR + 2>(x);
+    x += lp_dpp<ROR + 1>(x);
+    if constexpr (L == 64) {
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+    }
+    return x;
+}
+
 // the statistics of all lanes' columns together
 __device__ __forceinline__ LpStat lp_wave_join(LpStat s, LpFactor c)
 {
-    float m = s.m;
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    lp_raise(s, m, c);
-    for (int d = 1; d < 64; d <<= 1) {
-        s.l += __shfl_xor(s.l, d);
-        s.e += __shfl_xor(s.e, d);
-    }
+    lp_raise(s, lp_max<64>(s.m), c);
+    s.l = lp_sum<64>(s.l);
+    s.e = lp_sum<64>(s.e);
     return s;
 }
 
-// One wavefront's best columns, best first, one per lane: larger logit, then lower column.
+// Sixteen lanes' values in descending order (a bitonic network: every step keeps the larger of two lanes' values in the lower).
+__device__ __forceinline__ float lp_sort16(float x, int lane)
+{
+    const float b0 = lane & 1 ? -INFINITY : INFINITY, b1 = lane & 2 ? -INFINITY : INFINITY, b2 = lane & 4 ? -INFINITY : INFINITY,
+                b3 = lane & 8 ? -INFINITY : INFINITY;
+    // med3 with +inf is the maximum, with -inf the minimum
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<XOR1>(x), b0);
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<XOR3>(x), b1);
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<XOR1>(x), b0);
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<HALF_MIRROR>(x), b2);
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<XOR2>(x), b1);
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<XOR1>(x), b0);
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<MIRROR>(x), b3);
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<XOR3>(lp_dpp<HALF_MIRROR>(x)), b2);
+    x = __builtin_amdgcn_fmed3f(x, lp_dpp<XOR2>(x), b1);
+    return __builtin_amdgcn_fmed3f(x, lp_dpp<XOR1>(x), b0);
+}
+
+// The top-th largest of a group's L lanes' own maxima (a lane without columns: -inf): at least `top` columns reach it.
+// -FLT_MAX if there are none.
+template <int L> __device__ __forceinline__ float lp_threshold(float lane_max, int top, int lane)
+{
+    float s = lp_sort16(lane_max, lane & 15);
+    if constexpr (L == 64) {
+        // two sorted halves, one of them turned round, make a bitonic sequence: merged in log2 steps
+        const float b0 = lane & 1 ? -INFINITY : INFINITY, b1 = lane & 2 ? -INFINITY : INFINITY, b2 = lane & 4 ? -INFINITY : INFINITY,
+                    b3 = lane & 8 ? -INFINITY : INFINITY, b4 = lane & 16 ? -INFINITY : INFINITY, b5 = lane & 32 ? -INFINITY : INFINITY;
+        auto merge16 = [&] {
+            s = __builtin_amdgcn_fmed3f(s, lp_dpp<ROR + 8>(s), b3);
+            s = __builtin_amdgcn_fmed3f(s, lp_dpp<XOR3>(lp_dpp<HALF_MIRROR>(s)), b2);
+            s = __builtin_amdgcn_fmed3f(s, lp_dpp<XOR2>(s), b1);
+            s = __builtin_amdgcn_fmed3f(s, lp_dpp<XOR1>(s), b0);
+        };
+        s = __builtin_amdgcn_fmed3f(s, __shfl_xor(s, 31), b4);
+        merge16();
+        s = __builtin_amdgcn_fmed3f(s, __shfl_xor(s, 63), b5);
+        s = __builtin_amdgcn_fmed3f(s, __shfl_xor(s, 16), b4);
+        merge16();
+    }
+    return fmaxf(__shfl(s, (lane & (64 - L)) + top - 1), -FLT_MAX);
+}
+
+// (v, i) comes before (w, j): larger logit, then lower column
+__device__ __forceinline__ bool lp_before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+
+constexpr int LP_NONE = 0x40000000;        // columns from here on stand for "no column" (with v = -inf): cols <= 2^30
+
+// How many of a group's L entries (one per lane, no two the same) come before the lane's own; L = 64: of the first `count`.
+template <int L> __device__ __forceinline__ int lp_rank(float v, int i, int count)
+{
+    int rank = 0;
+    if constexpr (L == 16) {
+        float w = v;
+        int j = i;
+#pragma unroll
+        for (int k = 1; k < 16; k++) {
+            w = lp_dpp<ROR + 1>(w);
+            j = lp_dpp<ROR + 1>(j);
+            rank += lp_before(w, j, v, i);
+        }
+    } else {
+        for (int k = 0; k < count; k++) {
+            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k));
+            const int j = __builtin_amdgcn_readlane(i, k);
+            rank += lp_before(w, j, v, i);
+        }
+    }
+    return rank;
+}
+
+// One wavefront's best columns, best first, one per lane.
 struct LpList {
     float v = -INFINITY;
-    int i = 0x7fffffff;
+    int i = LP_NONE;
 };
 
 __device__ __forceinline__ void lp_insert(LpList& t, float cv, int ci, int lane)
 {
-    const unsigned long long before = __ballot(t.v > cv || (t.v == cv && t.i < ci));
+    const unsigned long long before = __ballot(lp_before(t.v, t.i, cv, ci));
     const int pos = __popcll(before);
     const float sv = __shfl_up(t.v, 1);
     const int si = __shfl_up(t.i, 1);
     if (lane == pos) { t.v = cv; t.i = ci; }
     else if (lane > pos) { t.v = sv; t.i = si; }
+}
+
+__device__ __forceinline__ void lp_wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
 struct LpArgs {
@@ -94,65 +198,363 @@ struct LpArgs {
     int cols;
 };
 
-// a row's outputs from its statistics (one wavefront; `t`: its list, best first)
-template <int E>
-__device__ __forceinline__ void lp_finish(const LpArgs& A, long row, LpStat s, const LpList& t, int lane)
+
+// lse, entropy and the given action's log probability of a row (one lane)
+template <int E> __device__ __forceinline__ void lp_write_row(const LpArgs& A, long row, const LpStat& s, float logl)
 {
     using raw = typename Elem<E>::raw;
     const bool none = s.l == 0.0f;                               // no allowed column
-    const float logl = logf(s.l);
-    const float lse = none ? -INFINITY : __builtin_amdgcn_fmed3f(lp_times(s.m, A.inv_t), -FLT_MAX, FLT_MAX) + logl;
-    if (lane == 0) {
-        if (A.lse) A.lse[row] = lse;
-        if (A.entropy) A.entropy[row] = none ? 0.0f : logl - LN2 * (s.e / s.l);
-        if (A.logp) {
-            const int a = A.actions[row];
-            float r = 0.0f;
-            if (a >= A.cols) r = NAN;
-            else if (a >= 0) {
-                const float x = elem_to_float<E>(((const raw*)A.x)[row * A.xstride + a]);
-                const bool there = x != -INFINITY && (!A.valid || A.valid[row * A.vstride + a]);
-                r = there ? lp_times(x - s.m, A.inv_t) - logl : -INFINITY;
+    if (A.lse) A.lse[row] = none ? -INFINITY : __builtin_amdgcn_fmed3f(lp_times(s.m, A.inv_t), -FLT_MAX, FLT_MAX) + logl;
+    if (A.entropy) A.entropy[row] = none ? 0.0f : logl - LN2 * (s.e / s.l);
+    if (A.logp) {
+        const int a = A.actions[row];
+        float r = 0.0f;
+        if (a >= A.cols) r = NAN;
+        else if (a >= 0) {
+            const float x = elem_to_float<E>(((const raw*)A.x)[row * A.xstride + a]);
+            const bool there = x != -INFINITY && (!A.valid || A.valid[row * A.vstride + a]);
+            r = there ? lp_times(x - s.m, A.inv_t) - logl : -INFINITY;
+        }
+        A.logp[row] = r;
+    }
+}
+__device__ __forceinline__ void lp_write_top(const LpArgs& A, long row, int rank, float v, int i, const LpStat& s, float logl)
+{
+    const bool some = i < LP_NONE;
+    A.top_actions[row * A.top + rank] = some ? i : -1;
+    A.top_logp[row * A.top + rank] = some ? lp_times(v - s.m, A.inv_t) - logl : -INFINITY;
+}
+
+// ---- short rows: all of a row in the registers of L lanes, NV vectors of V columns each; lane l's are (q L + l) V .. + V; the
+// first FULL vectors of every lane lie within the row for sure ----
+//
+// The alternatives: T = lp_threshold of the lanes' maxima leaves few candidates (for 8 of 362 columns about 11).  The row goes to
+// LDS, every lane looks up its candidates there (a bit each), one lane takes each, and a candidate's place is the number of those
+// before it.  Where more than L remain (ties, masks that leave few columns to few lanes) the search is place by place: round r takes
+// the best column behind round r - 1's.
+
+// bit (N - 1 - k) for x[k] >= t
+template <int N> __device__ __forceinline__ unsigned lp_at_least(const float (&x)[N], float t)
+{
+    unsigned bits = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        // bits = 2 bits + (x[k] >= t): a compare and an add with its carry
+        asm("v_cmp_ge_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(bits) : "v"(x[k]), "v"(t) : "vcc");
+    }
+    return bits;
+}
+
+template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs A)
+{
+    using raw = typename Elem<E>::raw;
+    constexpr int N = NV * V;
+    __shared__ float lds_x[TOP ? 256 * N : 1];                   // lane by lane
+    __shared__ float lds_v[TOP ? 256 : 1];
+    __shared__ int lds_i[TOP ? 256 : 1];
+    const int lane = threadIdx.x & 63, sub = lane & (L - 1);
+    const int group = (threadIdx.x & ~(L - 1));                  // this group's first slot in LDS
+    const long mine_row = (long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const bool active = mine_row < A.rows;                   // (the lanes behind the last row work on it too, and write nothing)
+    const long row = active ? mine_row : A.rows - 1;
+    // All loads are issued before the first is used.  A vector that would pass the row's end starts cols - V (cols >= V) instead; its
+    // columns in front of the lane's own are another lane's.
+    const int last = A.cols - V;
+    float x[N];
+    {
+        const raw* p = (const raw*)A.x + row * A.xstride;
+        ElemVec<E, V> t[NV];
+#pragma unroll
+        for (int q = 0; q < NV; q++) __builtin_memcpy(&t[q], p + min((q * L + sub) * V, last), sizeof(t[q]));
+        if (A.valid) {
+            const uint8_t* valid = A.valid + row * A.vstride;
+            uint8_t ok[NV][V];
+#pragma unroll
+            for (int q = 0; q < NV; q++) __builtin_memcpy(ok[q], valid + min((q * L + sub) * V, last), V);
+#pragma unroll
+            for (int k = 0; k < N; k++) x[k] = ok[k / V][k % V] ? elem_to_float<E>(t[k / V].a[k % V]) : -INFINITY;
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) x[k] = elem_to_float<E>(t[k / V].a[k % V]);
+        }
+#pragma unroll
+        for (int q = 0; q < NV; q++) {
+            const int c = (q * L + sub) * V, cc = min(c, last);
+            if (q >= FULL) {
+#pragma unroll
+                for (int k = 0; k < V; k++) x[q * V + k] = cc + k >= c ? x[q * V + k] : -INFINITY;
             }
-            A.logp[row] = r;
         }
     }
-    if (lane < A.top) {
-        const bool some = t.v != -INFINITY;
-        A.top_actions[row * A.top + lane] = some ? t.i : -1;
-        A.top_logp[row * A.top + lane] = some ? lp_times(t.v - s.m, A.inv_t) - logl : -INFINITY;
+    float lane_max = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < N; k++) lane_max = fmaxf(lane_max, x[k]);
+    LpStat s;
+    s.m = fmaxf(lp_max<L>(lane_max), -FLT_MAX);
+#pragma unroll
+    for (int k = 0; k < N; k++) lp_add(s, x[k], A.c2);
+    s.l = lp_sum<L>(s.l);
+    s.e = lp_sum<L>(s.e);
+    const float logl = logf(s.l);
+    if (sub == 0 && active) lp_write_row<E>(A, row, s, logl);
+    if constexpr (TOP) {
+        float* mine_x = lds_x + threadIdx.x * N;
+#pragma unroll
+        for (int k = 0; k < N; k++) mine_x[k] = x[k];
+        const float T = lp_threshold<L>(lane_max, A.top, lane);
+        unsigned bits = lp_at_least(x, T);
+        const int mine = __popc(bits);
+        int upto = mine;                                     // candidates of the lanes up to this one
+        for (int d = 1; d < L; d <<= 1) {
+            const int other = __shfl_up(upto, d, L);
+            upto += sub >= d ? other : 0;
+        }
+        int count = __shfl(upto, L - 1, L);
+        if constexpr (L == 64) count = __builtin_amdgcn_readfirstlane(count);
+        lp_wave_sync();
+        if (!__any(count > L)) {
+            int at = group + upto - mine;
+            while (__any(bits != 0)) {
+                if (bits) {
+                    const int k = __clz(bits) - (32 - N);
+                    bits &= ~(0x80000000u >> __clz(bits));
+                    lds_v[at] = mine_x[k];
+                    lds_i[at++] = min(((k / V) * L + sub) * V, last) + k % V;
+                }
+            }
+            lp_wave_sync();
+            const bool some = sub < count;
+            const float v = some ? lds_v[group + sub] : -INFINITY;
+            const int i = some ? lds_i[group + sub] : LP_NONE + sub;
+            int rank = lp_rank<L>(v, i, L == 64 ? count : L);
+            if (L == 64 && !some) rank = sub;                // behind all candidates
+            if (active && rank < A.top) lp_write_top(A, row, rank, v, i, s, logl);
+        } else {
+            float pv = INFINITY;                             // the place before
+            int pi = -1;
+            for (int r = 0; r < A.top; r++) {
+                float v = -INFINITY;
+                int i = LP_NONE;
+#pragma nounroll
+                for (int k = 0; k < N; k++) {
+                    const float w = mine_x[k];
+                    const int c = min(((k / V) * L + sub) * V, last) + k % V;
+                    if (w != -INFINITY && lp_before(pv, pi, w, c) && lp_before(w, c, v, i)) {
+                        v = w;
+                        i = c;
+                    }
+                }
+                for (int d = 1; d < L; d <<= 1) {
+                    const float w = __shfl_xor(v, d);
+                    const int j = __shfl_xor(i, d);
+                    if (lp_before(w, j, v, i)) { v = w; i = j; }
+                }
+                if (sub == 0 && active) lp_write_top(A, row, r, v, i, s, logl);
+                pv = v;
+                pi = i;
+            }
+        }
     }
 }
 
-// One wavefront per row.
-template <int E> __global__ __launch_bounds__(256) void k_logprobs(LpArgs A)
+// ---- long rows: a workgroup takes a segment of a row, each wavefront every fourth tile of it ----
+//
+// A wavefront keeps its list of alternatives across its lanes: the first tile's by threshold and rank as above, later columns only
+// where they beat the last one listed (k ln(n / k) of n, in random order), one insertion each.  A tile's columns come after all
+// earlier tiles', so only those strictly better than the last alternative of the tiles before can enter.
+constexpr int LP_E = 16;                                   // columns per lane and tile
+constexpr int LP_TILE = 64 * LP_E;
+constexpr int LP_SPLITS = 64;                              // at most: one list per lane when they are joined
+
+struct LpPart {                                            // a segment's result in the workspace
+    float m, l, e, pad;
+};
+
+// Sorted lists of `top` entries, list l at (lv, li) + l * top (one wavefront, lists <= 64): the best entries, best first, on the lanes
+__device__ __forceinline__ LpList lp_merge(const float* lv, const int* li, int lists, int top, int lane)
 {
-    using raw = typename Elem<E>::raw;
-    const int lane = threadIdx.x & 63;
-    for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < A.rows; row += (long)gridDim.x * 4) {
-    const raw* x = (const raw*)A.x + row * A.xstride;
-    const uint8_t* valid = A.valid ? A.valid + row * A.vstride : nullptr;
-    LpStat s;
-    LpList t;
-    float worst = -INFINITY;                        // the last alternative listed so far: later columns must beat it
-    for (int base = 0; base < A.cols; base += 64) {
-        const int c = base + lane;
-        const bool in = c < A.cols;
-        const float v = in && (!valid || valid[c]) ? elem_to_float<E>(x[c]) : -INFINITY;
-        if (v > s.m) lp_raise(s, v, A.c2);
-        lp_add(s, v, A.c2);
-        if (A.top) {
-            unsigned long long better = __ballot(v > worst);
-            while (better) {
-                const int src = __ffsll((long long)better) - 1;
-                better &= better - 1;
-                lp_insert(t, __shfl(v, src), base + src, lane);
-            }
-            worst = __shfl(t.v, A.top - 1);
+    LpList out;
+    int at = 0;
+    float v = lane < lists ? lv[lane * top] : -INFINITY;
+    int i = lane < lists ? li[lane * top] : LP_NONE + lane;
+    for (int r = 0; r < top; r++) {
+        float bv = v;
+        int bi = i;
+        for (int d = 1; d < lists; d <<= 1) {
+            const float w = __shfl_xor(bv, d);
+            const int j = __shfl_xor(bi, d);
+            if (lp_before(w, j, bv, bi)) { bv = w; bi = j; }
+        }
+        bv = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(bv)));
+        bi = __builtin_amdgcn_readfirstlane(bi);
+        if (bi >= LP_NONE) break;                          // nothing left
+        if (lane == r) { out.v = bv; out.i = bi; }
+        if (i == bi) {                                     // (columns differ: one lane)
+            at++;
+            v = at < top ? lv[lane * top + at] : -INFINITY;
+            i = at < top ? li[lane * top + at] : LP_NONE + lane;
         }
     }
+    return out;
+}
+
+template <int E, bool TOP>
+__global__ __launch_bounds__(256) void k_logprobs_long(LpArgs A, int splits, int segment, LpPart* __restrict__ parts, float* __restrict__ part_v,
+                                                       int* __restrict__ part_i)
+{
+    using raw = typename Elem<E>::raw;
+    constexpr int V = E == 0 ? 4 : 8, NV = LP_E / V;
+    __shared__ float lds_v[TOP ? 256 : 1];
+    __shared__ int lds_i[TOP ? 256 : 1];
+    __shared__ LpPart lds_s[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (long unit = blockIdx.x; unit < A.rows * splits; unit += gridDim.x) {
+        const long row = unit / splits;
+        const int split = (int)(unit - row * splits);
+        const int c0 = split * segment, c1 = min(A.cols, c0 + segment);
+        const raw* p = (const raw*)A.x + row * A.xstride;
+        const uint8_t* valid = A.valid ? A.valid + row * A.vstride : nullptr;
+        LpStat s;
+        LpList t;
+        float worst = -INFINITY;
+        bool first = true;
+        for (int base = c0 + wave * LP_TILE; base < c1; base += 4 * LP_TILE) {
+            float x[LP_E];
+            if (base + LP_TILE <= c1) {
+#pragma unroll
+                for (int q = 0; q < NV; q++) {
+                    const int c = base + (q * 64 + lane) * V;
+                    float u[V];
+                    elem_load<E, V>(p + c, u);
+#pragma unroll
+                    for (int k = 0; k < V; k++) x[q * V + k] = u[k];
+                }
+                if (valid) {
+#pragma unroll
+                    for (int q = 0; q < NV; q++) {
+                        uint8_t ok[V];
+                        __builtin_memcpy(ok, valid + base + (q * 64 + lane) * V, V);
+#pragma unroll
+                        for (int k = 0; k < V; k++) x[q * V + k] = ok[k] ? x[q * V + k] : -INFINITY;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < LP_E; k++) {
+                    const int c = base + ((k / V) * 64 + lane) * V + k % V;
+                    x[k] = c < c1 && (!valid || valid[c]) ? elem_to_float<E>(p[c]) : -INFINITY;
+                }
+            }
+            float lane_max = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < LP_E; k++) lane_max = fmaxf(lane_max, x[k]);
+            lp_raise(s, fmaxf(s.m, lane_max), A.c2);
+#pragma unroll
+            for (int k = 0; k < LP_E; k++) lp_add(s, x[k], A.c2);
+            if constexpr (TOP) {
+                bool listed = false;
+                float bar = worst;                         // columns above it may enter
+                if (first) {
+                    const float T = lp_threshold<64>(lane_max, A.top, lane);
+                    const int mine = __popc(lp_at_least(x, T));
+                    int upto = mine;
+                    for (int d = 1; d < 64; d <<= 1) {
+                        const int other = __shfl_up(upto, d);
+                        upto += lane >= d ? other : 0;
+                    }
+                    const int count = __builtin_amdgcn_readlane(upto, 63);
+                    if (count <= 64) {
+                        int at = wave * 64 + upto - mine;
+#pragma unroll
+                        for (int k = 0; k < LP_E; k++)
+                            if (x[k] >= T) {
+                                lds_v[at] = x[k];
+                                lds_i[at++] = base + ((k / V) * 64 + lane) * V + k % V;
+                            }
+                        lp_wave_sync();
+                        const bool some = lane < count;
+                        const float v = some ? lds_v[wave * 64 + lane] : -INFINITY;
+                        const int i = some ? lds_i[wave * 64 + lane] : LP_NONE + lane;
+                        lp_wave_sync();
+                        const int rank = some ? lp_rank<64>(v, i, count) : lane;
+                        lds_v[wave * 64 + rank] = v;
+                        lds_i[wave * 64 + rank] = i;
+                        lp_wave_sync();
+                        t.v = lds_v[wave * 64 + lane];
+                        t.i = lds_i[wave * 64 + lane];
+                        lp_wave_sync();
+                        listed = true;
+                    }
+                    bar = T == -FLT_MAX ? -INFINITY : nextafterf(T, -INFINITY);
+                    first = false;
+                }
+                if (!listed && __any(lane_max > bar)) {
+#pragma unroll
+                    for (int k = 0; k < LP_E; k++) {
+                        unsigned long long better = __ballot(x[k] > bar);
+                        while (better) {
+                            const int src = __ffsll((long long)better) - 1;
+                            better &= better - 1;
+                            lp_insert(t, __shfl(x[k], src), base + ((k / V) * 64 + src) * V + k % V, lane);
+                        }
+                    }
+                }
+                worst = __shfl(t.v, A.top - 1);
+            }
+        }
+        s = lp_wave_join(s, A.c2);
+        __syncthreads();                                   // all waves' first tiles are done with the LDS arrays
+        if (lane == 0) lds_s[wave] = LpPart{ s.m, s.l, s.e, 0.0f };
+        if (TOP && lane < A.top) {
+            lds_v[wave * A.top + lane] = t.v;
+            lds_i[wave * A.top + lane] = t.i;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            s = LpStat();
+            if (lane < 4) {
+                s.m = lds_s[lane].m;
+                s.l = lds_s[lane].l;
+                s.e = lds_s[lane].e;
+            }
+            s = lp_wave_join(s, A.c2);
+            if constexpr (TOP) t = lp_merge(lds_v, lds_i, 4, A.top, lane);
+            if (splits == 1) {
+                const float logl = logf(s.l);
+                if (lane == 0) lp_write_row<E>(A, row, s, logl);
+                if (TOP && lane < A.top) lp_write_top(A, row, lane, t.v, t.i, s, logl);
+            } else {
+                if (lane == 0) parts[unit] = LpPart{ s.m, s.l, s.e, 0.0f };
+                if (TOP && lane < A.top) {
+                    part_v[unit * A.top + lane] = t.v;
+                    part_i[unit * A.top + lane] = t.i;
+                }
+            }
+        }
+        __syncthreads();                                   // the next unit's first tiles write the LDS arrays
+    }
+}
+
+// the segments of a row together: one wavefront per row
+template <int E, bool TOP>
+__global__ __launch_bounds__(64) void k_logprobs_join(LpArgs A, int splits, const LpPart* __restrict__ parts, const float* __restrict__ part_v,
+                                                      const int* __restrict__ part_i)
+{
+    const long row = blockIdx.x;
+    const int lane = threadIdx.x;
+    LpStat s;
+    if (lane < splits) {
+        const LpPart q = parts[row * splits + lane];
+        s.m = q.m;
+        s.l = q.l;
+        s.e = q.e;
+    }
     s = lp_wave_join(s, A.c2);
-    lp_finish<E>(A, row, s, t, lane);
+    const float logl = logf(s.l);
+    if (lane == 0) lp_write_row<E>(A, row, s, logl);
+    if constexpr (TOP) {
+        const LpList t = lp_merge(part_v + row * splits * A.top, part_i + row * splits * A.top, splits, A.top, lane);
+        if (lane < A.top) lp_write_top(A, row, lane, t.v, t.i, s, logl);
     }
 }
 
@@ -208,13 +610,81 @@ static LpFactor lp_factor(double c)
         default: { constexpr int E = 2; __VA_ARGS__; } break;        \
     }
 
+constexpr int LP_SHORT = 1024;                      // longest row that stays in a wavefront's registers
+
+// Segments of a long row: enough of them that the rows' fill the GPU, none shorter than four tiles
+static int lp_splits(int64_t rows, int cols)
+{
+    if (cols <= LP_SHORT) return 1;
+    const int64_t want = (512 + rows - 1) / rows, most = std::max(1, cols / (4 * LP_TILE));
+    return (int)std::min<int64_t>({ want, most, LP_SPLITS });
+}
+
+int64_t action_logprobs_workspace(int64_t rows, int cols, int top)
+{
+    const int64_t splits = lp_splits(std::max<int64_t>(rows, 1), cols);
+    return splits == 1 ? 0 : rows * splits * (int64_t)(sizeof(LpPart) + 8 * top);
+}
+
+constexpr long LP_GRID = 1 << 22;                   // workgroups per launch
+
+template <int E, int L, int V, int NV, int FULL> static void lp_launch_short(LpArgs A, hipStream_t st)
+{
+    const long per = 256 / L, all = A.rows;
+    for (long row = 0; row < all; row += LP_GRID * per) {
+        A.rows = std::min(all - row, LP_GRID * per);
+        const unsigned grid = (unsigned)((A.rows + per - 1) / per);
+        if (A.top) k_logprobs_short<E, L, V, NV, FULL, true><<<grid, 256, 0, st>>>(A);
+        else k_logprobs_short<E, L, V, NV, FULL, false><<<grid, 256, 0, st>>>(A);
+        A.x = (const char*)A.x + A.rows * A.xstride * (long)sizeof(typename Elem<E>::raw);
+        if (A.valid) A.valid += A.rows * A.vstride;
+        if (A.actions) A.actions += A.rows;
+        if (A.logp) A.logp += A.rows;
+        if (A.entropy) A.entropy += A.rows;
+        if (A.lse) A.lse += A.rows;
+        if (A.top) {
+            A.top_actions += A.rows * A.top;
+            A.top_logp += A.rows * A.top;
+        }
+    }
+}
+
+template <int E> static void lp_launch(const LpArgs& A, void* workspace, hipStream_t st)
+{
+    // sixteen lanes per row: up to 384 columns and eight alternatives (of sixteen lanes' maxima the eighth is still a sharp
+    // threshold); else a wavefront per row
+    if (A.cols <= 384 && A.top <= 8) {
+        if (A.cols <= 32) lp_launch_short<E, 16, 1, 2, 0>(A, st);
+        else if (A.cols <= 64) lp_launch_short<E, 16, 4, 1, 0>(A, st);
+        else if (A.cols <= 128) lp_launch_short<E, 16, 4, 2, 1>(A, st);
+        else if (A.cols <= 192) lp_launch_short<E, 16, 4, 3, 2>(A, st);
+        else lp_launch_short<E, 16, 4, 6, 3>(A, st);
+    } else if (A.cols <= LP_SHORT) {
+        if (A.cols <= 128) lp_launch_short<E, 64, 1, 2, 0>(A, st);
+        else if (A.cols <= 384) lp_launch_short<E, 64, 1, 6, 2>(A, st);
+        else lp_launch_short<E, 64, 1, 16, 6>(A, st);
+    } else {
+        const int splits = lp_splits(A.rows, A.cols);
+        const int segment = ((A.cols + splits - 1) / splits + LP_TILE - 1) / LP_TILE * LP_TILE;
+        LpPart* parts = (LpPart*)workspace;
+        float* pv = (float*)(parts + A.rows * splits);
+        int* pi = (int*)(pv + A.rows * splits * A.top);
+        const unsigned grid = (unsigned)std::min<long>(A.rows * splits, 1 << 20);
+        if (A.top) k_logprobs_long<E, true><<<grid, 256, 0, st>>>(A, splits, segment, parts, pv, pi);
+        else k_logprobs_long<E, false><<<grid, 256, 0, st>>>(A, splits, segment, parts, pv, pi);
+        if (splits == 1) return;
+        if (A.top) k_logprobs_join<E, true><<<(unsigned)A.rows, 64, 0, st>>>(A, splits, parts, pv, pi);
+        else k_logprobs_join<E, false><<<(unsigned)A.rows, 64, 0, st>>>(A, splits, parts, pv, pi);
+    }
+}
+
 int launch_action_logprobs(const void* logits, int elem, int64_t stride, const uint8_t* valid, int64_t valid_stride, const int32_t* actions,
                            double temperature, int top, float* logp, float* entropy, float* lse, int32_t* top_actions, float* top_logp,
-                           int64_t rows, int cols, hipStream_t st)
+                           int64_t rows, int cols, void* workspace, hipStream_t st)
 {
-    const LpArgs A{ logits, (long)stride, valid, (long)valid_stride, actions, lp_factor(1.0 / temperature), lp_factor(1.44269504088896340736 / temperature), top, logp, entropy, lse, top_actions, top_logp,
-                    (long)rows, cols };
-    LP_DISPATCH(elem, k_logprobs<E><<<(unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 20), 256, 0, st>>>(A));
+    const LpArgs A{ logits, (long)stride, valid, (long)valid_stride, actions, lp_factor(1.0 / temperature),
+                    lp_factor(1.44269504088896340736 / temperature), top, logp, entropy, lse, top_actions, top_logp, (long)rows, cols };
+    LP_DISPATCH(elem, lp_launch<E>(A, workspace, st));
     GOAI_HIP_CHECK(hipGetLastError());
     return GOAI_OK;
 }

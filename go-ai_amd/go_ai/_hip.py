@@ -75,7 +75,8 @@ _SIGNATURES = {
     "goai_train_params": [c_void_p, ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64)],
     "goai_train_sync_inference": [c_void_p],
     "goai_action_logprobs": [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_double, c_int, c_void_p, c_void_p, c_void_p,
-                             c_void_p, c_void_p, c_int64, c_int],
+                             c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64],
+    "goai_action_logprobs_workspace": [c_int64, c_int, c_int],
     "goai_action_logprobs_grad": [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_double, c_void_p, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_int64, c_int64, c_int],
     "goai_adamw_state_elems": [c_int, c_void_p],
@@ -96,7 +97,7 @@ _SIGNATURES = {
 
 for _name, _args in _SIGNATURES.items():
     _fn = getattr(lib, _name)          # AttributeError here = library older than this binding
-    _fn.restype = c_int64 if _name == "goai_adamw_state_elems" else c_int
+    _fn.restype = c_int64 if _name in ("goai_adamw_state_elems", "goai_action_logprobs_workspace") else c_int
     _fn.argtypes = _args
 
 

@@ -213,6 +213,7 @@ class Context:
         return x
 
     LOGPROBS_MAX_TOP = 64
+    LOGPROBS_SHORT = 1024        # up to so many columns goai_action_logprobs needs no workspace
 
     def action_logprobs(self, logits, actions=None, valid=None, temperature=1.0, top=0):
         """goai_action_logprobs: log probabilities of `actions` [rows] under softmax(logits / temperature) over the columns with
@@ -235,9 +236,12 @@ class Context:
         if a is None:
             logp = None
         if rows:
-            p = _hip.dptr
+            p, work, need = _hip.dptr, None, 0
+            if cols > self.LOGPROBS_SHORT:              # few long rows are split, and the parts joined
+                need = _hip.lib.goai_action_logprobs_workspace(rows, cols, top)
+                work = torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None
             _hip.check(_hip.lib.goai_action_logprobs(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), temperature, top, p(logp),
-                                                     p(entropy), p(lse), p(best), p(best_lp), rows, cols))
+                                                     p(entropy), p(lse), p(best), p(best_lp), rows, cols, p(work), need))
         return ActionLogprobs(logp, entropy, lse, best, best_lp)
 
     def action_logprobs_grad(self, logits, actions, lse, entropy=None, d_logp=None, d_entropy=None, valid=None, temperature=1.0, out=None):

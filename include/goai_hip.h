@@ -408,7 +408,10 @@ int goai_train_sync_inference(goai_ctx* ctx);
  * listed).  logp (with actions), entropy, lse may be NULL.  Sums are float32 whatever the logits' type. */
 int goai_action_logprobs(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid,
                          int64_t valid_stride, const int32_t* actions, double temperature, int top, float* logp, float* entropy,
-                         float* lse, int32_t* top_actions, float* top_logp, int64_t rows, int cols);
+                         float* lse, int32_t* top_actions, float* top_logp, int64_t rows, int cols, void* workspace,
+                         int64_t workspace_bytes);
+/* Bytes of DEVICE workspace (16-byte aligned, used during the call alone) for these sizes; 0: none (workspace may be NULL). */
+int64_t goai_action_logprobs_workspace(int64_t rows, int cols, int top);
 
 /* The gradient with respect to the logits of a loss whose gradients with respect to logp and entropy are d_logp and
  * d_entropy (float32 [rows]; either may be NULL: 0):

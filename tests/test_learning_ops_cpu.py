@@ -16,10 +16,11 @@ def err():
 
 
 def logprobs(**k):
-    a = dict(logits=64, elem=0, stride=82, valid=None, vstride=0, actions=64, t=1.0, top=0, logp=64, ent=64, lse=64, ta=None, tl=None, rows=4, cols=82)
+    a = dict(logits=64, elem=0, stride=82, valid=None, vstride=0, actions=64, t=1.0, top=0, logp=64, ent=64, lse=64, ta=None, tl=None, rows=4, cols=82,
+             work=None, bytes=0)
     a.update(k)
     return lib.goai_action_logprobs(None, a["logits"], a["elem"], a["stride"], a["valid"], a["vstride"], a["actions"], a["t"], a["top"], a["logp"],
-                                    a["ent"], a["lse"], a["ta"], a["tl"], a["rows"], a["cols"])
+                                    a["ent"], a["lse"], a["ta"], a["tl"], a["rows"], a["cols"], a["work"], a["bytes"])
 
 
 @pytest.mark.parametrize("bad,message", [
@@ -28,9 +29,23 @@ def logprobs(**k):
     (dict(t=-1.0), "temperature"), (dict(logits=None), "logits"), (dict(logits=66), "aligned"), (dict(logits=65, elem=1), "aligned"),
     (dict(stride=81), "stride"), (dict(stride=-82), "stride"), (dict(valid=64, vstride=5), "stride"), (dict(top=65), "top"), (dict(top=-1), "top"),
     (dict(top=3), "top_actions"), (dict(top=3, ta=64), "top_logp"), (dict(actions=None), "actions"), (dict(rows=0, logits=None), "ctx is NULL"),
+    (dict(rows=3, cols=200_000, stride=200_000), "workspace"), (dict(rows=3, cols=200_000, stride=200_000, work=64, bytes=64), "workspace"),
+    (dict(rows=3, cols=200_000, stride=200_000, work=72, bytes=1 << 30), "workspace"),
+    (dict(rows=3, cols=200_000, stride=200_000, work=64, bytes=1 << 30), "ctx is NULL"),
 ])
 def test_logprobs(bad, message):
     assert logprobs(**bad) == -1 and message in err()
+
+
+def test_logprobs_workspace():
+    f = lib.goai_action_logprobs_workspace
+    assert f(5, 82, 64) == 0 and f(0, 1 << 30, 64) == 0 and f(1, 1024, 64) == 0
+    for rows in (1, 3, 511, 512, 100_000):
+        for cols in (1025, 4097, 70_001, 1 << 30):
+            for top in (0, 64):
+                need = f(rows, cols, top)
+                assert 0 <= need <= rows * 64 * (16 + 8 * top) and (need == 0 or rows < 512)
+    assert f(-1, 82, 0) == -1 and f(1, 0, 0) == -1 and f(1, 82, 65) == -1
 
 
 def grad(**k):
