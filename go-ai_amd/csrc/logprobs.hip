@@ -132,6 +132,74 @@ template <int L> __device__ __forceinline__ float lp_threshold(float lane_max, i
     return fmaxf(__shfl(s, (lane & (64 - L)) + top - 1), -FLT_MAX);
 }
 
+// bit (N - 1 - k) for x[k] >= t
+template <int N> __device__ __forceinline__ unsigned lp_at_least(const float (&x)[N], float t)
+{
+    unsigned bits = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        // bits = 2 bits + (x[k] >= t): a compare and an add with its carry
+        asm("v_cmp_ge_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(bits) : "v"(x[k]), "v"(t) : "vcc");
+    }
+    return bits;
+}
+
+template <int L> __device__ __forceinline__ int lp_count(int n)
+{
+    n += lp_dpp<ROR + 8>(n);
+    n += lp_dpp<ROR + 4>(n);
+    n += lp_dpp<ROR + 2>(n);
+    n += lp_dpp<ROR + 1>(n);
+    if constexpr (L == 64) {
+        n += __shfl_xor(n, 16);
+        n += __shfl_xor(n, 32);
+    }
+    return n;
+}
+
+// floats as integers of the same order, and back
+__device__ __forceinline__ int lp_key(int bits) { return bits ^ ((bits >> 31) & 0x7fffffff); }
+
+// The candidates of a group of L lanes for its `top` best columns: at least `top` of them (all, if there are fewer), bits as in
+// lp_at_least, `count` in the group; at most L unless several columns share the top-th value.
+// The first threshold, lp_threshold, is sharp while a lane seldom holds two of the best; where it leaves more than L, halving
+// the range between it and the largest value does (3.5 % of the wavefronts for 8 of 362 columns over 16 lanes, some 3 steps).
+template <int L, int N> __device__ __forceinline__ unsigned lp_candidates(const float (&x)[N], float lane_max, float most, int top, int lane, int& count)
+{
+    const float T = lp_threshold<L>(lane_max, top, lane);
+    unsigned bits = lp_at_least(x, T);
+    count = lp_count<L>(__popc(bits));
+    if (__any(count > L)) {
+        int lo = lp_key(__float_as_int(T)), hi = lp_key(__float_as_int(most)) + 1;       // enough columns reach lo, too few reach hi
+        for (int step = 0; step < 32 && __any(count > L && hi - lo > 1); step++) {
+            const int mid = (int)((unsigned)lo + (((unsigned)hi - (unsigned)lo) >> 1));
+            const unsigned b = lp_at_least(x, __int_as_float(lp_key(mid)));
+            const int n = lp_count<L>(__popc(b));
+            if (count > L) {
+                if (n >= top) {
+                    lo = mid;
+                    bits = b;
+                    count = n;
+                } else hi = mid;
+            }
+        }
+    }
+    if constexpr (L == 64) count = __builtin_amdgcn_readfirstlane(count);
+    return bits;
+}
+
+// the sum of n over the lanes of a group before this one
+template <int L> __device__ __forceinline__ int lp_before_me(int n, int sub)
+{
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) {
+        const int other = __shfl_up(upto, d, L);
+        upto += sub >= d ? other : 0;
+    }
+    return upto - n;
+}
+
 // (v, i) comes before (w, j): larger logit, then lower column
 __device__ __forceinline__ bool lp_before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
@@ -199,24 +267,25 @@ struct LpArgs {
 };
 
 
-// lse, entropy and the given action's log probability of a row (one lane)
-template <int E> __device__ __forceinline__ void lp_write_row(const LpArgs& A, long row, const LpStat& s, float logl)
+// The given action's logit, read early (its address waits for another load): NaN for an action beyond the row, -inf where the column
+// is not allowed, +inf (which no allowed finite logit is: a row with one is NaN anyway) for "no action".
+template <int E> __device__ __forceinline__ float lp_given(const LpArgs& A, long row)
 {
     using raw = typename Elem<E>::raw;
+    const int a = A.actions ? A.actions[row] : -1;
+    if (a >= A.cols) return NAN;
+    if (a < 0) return INFINITY;
+    const float x = elem_to_float<E>(((const raw*)A.x)[row * A.xstride + a]);
+    return A.valid && !A.valid[row * A.vstride + a] ? -INFINITY : x == INFINITY ? NAN : x;
+}
+
+// lse, entropy and the given action's log probability of a row (one lane)
+__device__ __forceinline__ void lp_write_row(const LpArgs& A, long row, const LpStat& s, float logl, float given)
+{
     const bool none = s.l == 0.0f;                               // no allowed column
     if (A.lse) A.lse[row] = none ? -INFINITY : __builtin_amdgcn_fmed3f(lp_times(s.m, A.inv_t), -FLT_MAX, FLT_MAX) + logl;
     if (A.entropy) A.entropy[row] = none ? 0.0f : logl - LN2 * (s.e / s.l);
-    if (A.logp) {
-        const int a = A.actions[row];
-        float r = 0.0f;
-        if (a >= A.cols) r = NAN;
-        else if (a >= 0) {
-            const float x = elem_to_float<E>(((const raw*)A.x)[row * A.xstride + a]);
-            const bool there = x != -INFINITY && (!A.valid || A.valid[row * A.vstride + a]);
-            r = there ? lp_times(x - s.m, A.inv_t) - logl : -INFINITY;
-        }
-        A.logp[row] = r;
-    }
+    if (A.logp) A.logp[row] = given == INFINITY ? 0.0f : given == -INFINITY ? -INFINITY : lp_times(given - s.m, A.inv_t) - logl;
 }
 __device__ __forceinline__ void lp_write_top(const LpArgs& A, long row, int rank, float v, int i, const LpStat& s, float logl)
 {
@@ -233,18 +302,6 @@ __device__ __forceinline__ void lp_write_top(const LpArgs& A, long row, int rank
 // before it.  Where more than L remain (ties, masks that leave few columns to few lanes) the search is place by place: round r takes
 // the best column behind round r - 1's.
 
-// bit (N - 1 - k) for x[k] >= t
-template <int N> __device__ __forceinline__ unsigned lp_at_least(const float (&x)[N], float t)
-{
-    unsigned bits = 0;
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-        // bits = 2 bits + (x[k] >= t): a compare and an add with its carry
-        asm("v_cmp_ge_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(bits) : "v"(x[k]), "v"(t) : "vcc");
-    }
-    return bits;
-}
-
 template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs A)
 {
     using raw = typename Elem<E>::raw;
@@ -260,6 +317,7 @@ template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_b
     // All loads are issued before the first is used.  A vector that would pass the row's end starts cols - V (cols >= V) instead; its
     // columns in front of the lane's own are another lane's.
     const int last = A.cols - V;
+    const float given = lp_given<E>(A, row);
     float x[N];
     {
         const raw* p = (const raw*)A.x + row * A.xstride;
@@ -296,24 +354,16 @@ template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_b
     s.l = lp_sum<L>(s.l);
     s.e = lp_sum<L>(s.e);
     const float logl = logf(s.l);
-    if (sub == 0 && active) lp_write_row<E>(A, row, s, logl);
+    if (sub == 0 && active) lp_write_row(A, row, s, logl, given);
     if constexpr (TOP) {
         float* mine_x = lds_x + threadIdx.x * N;
 #pragma unroll
         for (int k = 0; k < N; k++) mine_x[k] = x[k];
-        const float T = lp_threshold<L>(lane_max, A.top, lane);
-        unsigned bits = lp_at_least(x, T);
-        const int mine = __popc(bits);
-        int upto = mine;                                     // candidates of the lanes up to this one
-        for (int d = 1; d < L; d <<= 1) {
-            const int other = __shfl_up(upto, d, L);
-            upto += sub >= d ? other : 0;
-        }
-        int count = __shfl(upto, L - 1, L);
-        if constexpr (L == 64) count = __builtin_amdgcn_readfirstlane(count);
+        int count;
+        unsigned bits = lp_candidates<L>(x, lane_max, s.m, A.top, lane, count);
+        int at = group + lp_before_me<L>(__popc(bits), sub);
         lp_wave_sync();
         if (!__any(count > L)) {
-            int at = group + upto - mine;
             while (__any(bits != 0)) {
                 if (bits) {
                     const int k = __clz(bits) - (32 - N);
@@ -359,11 +409,12 @@ template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_b
 
 // ---- long rows: a workgroup takes a segment of a row, each wavefront every fourth tile of it ----
 //
-// A wavefront keeps its list of alternatives across its lanes: the first tile's by threshold and rank as above, later columns only
-// where they beat the last one listed (k ln(n / k) of n, in random order), one insertion each.  A tile's columns come after all
-// earlier tiles', so only those strictly better than the last alternative of the tiles before can enter.
+// A wavefront keeps its list of alternatives across its lanes.  A tile's columns come after all earlier tiles', so only those
+// strictly better than the last alternative listed can enter (k ln(n / k) of n, in random order): a few one by one, many -- the first
+// tile's, and those of rows that rise -- as a list of the tile's own that is merged in.
 constexpr int LP_E = 16;                                   // columns per lane and tile
 constexpr int LP_TILE = 64 * LP_E;
+constexpr int LP_FEW = 12;                                 // columns that enter a list one by one: some 60 cycles each, a list of their own 800
 constexpr int LP_SPLITS = 64;                              // at most: one list per lane when they are joined
 
 struct LpPart {                                            // a segment's result in the workspace
@@ -398,8 +449,18 @@ __device__ __forceinline__ LpList lp_merge(const float* lv, const int* li, int l
     return out;
 }
 
+// How many of a sorted list's `top` entries come before (v, i)
+__device__ __forceinline__ int lp_search(const float* lv, const int* li, int top, float v, int i)
+{
+    int at = 0;
+#pragma unroll
+    for (int d = 64; d; d >>= 1)
+        if (at + d <= top && lp_before(lv[at + d - 1], li[at + d - 1], v, i)) at += d;
+    return at;
+}
+
 template <int E, bool TOP>
-__global__ __launch_bounds__(256) void k_logprobs_long(LpArgs A, int splits, int segment, LpPart* __restrict__ parts, float* __restrict__ part_v,
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k_logprobs_long(LpArgs A, int splits, int segment, LpPart* __restrict__ parts, float* __restrict__ part_v,
                                                        int* __restrict__ part_i)
 {
     using raw = typename Elem<E>::raw;
@@ -408,140 +469,177 @@ __global__ __launch_bounds__(256) void k_logprobs_long(LpArgs A, int splits, int
     __shared__ int lds_i[TOP ? 256 : 1];
     __shared__ LpPart lds_s[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (long unit = blockIdx.x; unit < A.rows * splits; unit += gridDim.x) {
-        const long row = unit / splits;
-        const int split = (int)(unit - row * splits);
-        const int c0 = split * segment, c1 = min(A.cols, c0 + segment);
-        const raw* p = (const raw*)A.x + row * A.xstride;
-        const uint8_t* valid = A.valid ? A.valid + row * A.vstride : nullptr;
-        LpStat s;
-        LpList t;
-        float worst = -INFINITY;
-        bool first = true;
-        for (int base = c0 + wave * LP_TILE; base < c1; base += 4 * LP_TILE) {
-            float x[LP_E];
-            if (base + LP_TILE <= c1) {
+    const long unit = blockIdx.x;
+    const long row = unit / splits;
+    const int split = (int)(unit - row * splits);
+    const int c0 = split * segment, c1 = min(A.cols, c0 + segment);
+    const raw* p = (const raw*)A.x + row * A.xstride;
+    const uint8_t* valid = A.valid ? A.valid + row * A.vstride : nullptr;
+    const float given = splits == 1 ? lp_given<E>(A, row) : 0.0f;
+    LpStat s;
+    LpList t;
+    float worst = -INFINITY;                           // the last alternative of the tiles before
+    for (int base = c0 + wave * LP_TILE; base < c1; base += 4 * LP_TILE) {
+        float x[LP_E];
+        if (base + LP_TILE <= c1) {
+#pragma unroll
+            for (int q = 0; q < NV; q++) {
+                const int c = base + (q * 64 + lane) * V;
+                float u[V];
+                elem_load<E, V>(p + c, u);
+#pragma unroll
+                for (int k = 0; k < V; k++) x[q * V + k] = u[k];
+            }
+            if (valid) {
 #pragma unroll
                 for (int q = 0; q < NV; q++) {
-                    const int c = base + (q * 64 + lane) * V;
-                    float u[V];
-                    elem_load<E, V>(p + c, u);
+                    uint8_t ok[V];
+                    __builtin_memcpy(ok, valid + base + (q * 64 + lane) * V, V);
 #pragma unroll
-                    for (int k = 0; k < V; k++) x[q * V + k] = u[k];
-                }
-                if (valid) {
-#pragma unroll
-                    for (int q = 0; q < NV; q++) {
-                        uint8_t ok[V];
-                        __builtin_memcpy(ok, valid + base + (q * 64 + lane) * V, V);
-#pragma unroll
-                        for (int k = 0; k < V; k++) x[q * V + k] = ok[k] ? x[q * V + k] : -INFINITY;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < LP_E; k++) {
-                    const int c = base + ((k / V) * 64 + lane) * V + k % V;
-                    x[k] = c < c1 && (!valid || valid[c]) ? elem_to_float<E>(p[c]) : -INFINITY;
+                    for (int k = 0; k < V; k++) x[q * V + k] = ok[k] ? x[q * V + k] : -INFINITY;
                 }
             }
-            float lane_max = -INFINITY;
+        } else {
 #pragma unroll
-            for (int k = 0; k < LP_E; k++) lane_max = fmaxf(lane_max, x[k]);
-            lp_raise(s, fmaxf(s.m, lane_max), A.c2);
+            for (int k = 0; k < LP_E; k++) {
+                const int c = base + ((k / V) * 64 + lane) * V + k % V;
+                x[k] = c < c1 && (!valid || valid[c]) ? elem_to_float<E>(p[c]) : -INFINITY;
+            }
+        }
+        float lane_max = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < LP_E; k++) lp_add(s, x[k], A.c2);
-            if constexpr (TOP) {
-                bool listed = false;
-                float bar = worst;                         // columns above it may enter
-                if (first) {
-                    const float T = lp_threshold<64>(lane_max, A.top, lane);
-                    const int mine = __popc(lp_at_least(x, T));
-                    int upto = mine;
-                    for (int d = 1; d < 64; d <<= 1) {
-                        const int other = __shfl_up(upto, d);
-                        upto += lane >= d ? other : 0;
-                    }
-                    const int count = __builtin_amdgcn_readlane(upto, 63);
-                    if (count <= 64) {
-                        int at = wave * 64 + upto - mine;
+        for (int k = 0; k < LP_E; k++) lane_max = fmaxf(lane_max, x[k]);
+        lp_raise(s, fmaxf(s.m, lane_max), A.c2);
 #pragma unroll
-                        for (int k = 0; k < LP_E; k++)
-                            if (x[k] >= T) {
-                                lds_v[at] = x[k];
-                                lds_i[at++] = base + ((k / V) * 64 + lane) * V + k % V;
-                            }
-                        lp_wave_sync();
-                        const bool some = lane < count;
-                        const float v = some ? lds_v[wave * 64 + lane] : -INFINITY;
-                        const int i = some ? lds_i[wave * 64 + lane] : LP_NONE + lane;
-                        lp_wave_sync();
-                        const int rank = some ? lp_rank<64>(v, i, count) : lane;
-                        lds_v[wave * 64 + rank] = v;
-                        lds_i[wave * 64 + rank] = i;
-                        lp_wave_sync();
-                        t.v = lds_v[wave * 64 + lane];
-                        t.i = lds_i[wave * 64 + lane];
-                        lp_wave_sync();
-                        listed = true;
-                    }
-                    bar = T == -FLT_MAX ? -INFINITY : nextafterf(T, -INFINITY);
-                    first = false;
+        for (int k = 0; k < LP_E; k++) lp_add(s, x[k], A.c2);
+        if constexpr (TOP) {
+            if (__any(lane_max > worst)) {
+                unsigned enter = 0xffffffffu;              // columns that may enter, if above the last one listed
+                int count = 0;
+                // more than a few: the tile's own list, by threshold and rank as a short row's, and the two lists merged
+                bool one_by_one = lp_count<64>(__popc(lp_at_least(x, fmaxf(worst, -FLT_MAX)))) <= LP_FEW;
+                if (!one_by_one) {
+                    enter = lp_candidates<64>(x, lane_max, lp_max<64>(lane_max), A.top, lane, count);
+                    one_by_one = count > 64;               // (ties)
                 }
-                if (!listed && __any(lane_max > bar)) {
+                if (one_by_one) {
 #pragma unroll
                     for (int k = 0; k < LP_E; k++) {
-                        unsigned long long better = __ballot(x[k] > bar);
+                        if (k && k % V == 0) worst = __shfl(t.v, A.top - 1);       // the next vectors' columns come after these
+                        unsigned long long better = __ballot(x[k] > worst && (enter & (1u << (LP_E - 1 - k))));
                         while (better) {
                             const int src = __ffsll((long long)better) - 1;
                             better &= better - 1;
                             lp_insert(t, __shfl(x[k], src), base + ((k / V) * 64 + src) * V + k % V, lane);
                         }
                     }
+                } else {
+                    float* wv = lds_v + wave * 64;
+                    int* wi = lds_i + wave * 64;
+                    int at = lp_before_me<64>(__popc(enter), lane);
+#pragma unroll
+                    for (int k = 0; k < LP_E; k++)
+                        if (enter & (1u << (LP_E - 1 - k))) {
+                            wv[at] = x[k];
+                            wi[at++] = base + ((k / V) * 64 + lane) * V + k % V;
+                        }
+                    lp_wave_sync();
+                    const bool some = lane < count;
+                    float v = some ? wv[lane] : -INFINITY;
+                    int i = some ? wi[lane] : LP_NONE + 64 + lane;
+                    lp_wave_sync();
+                    int rank = some ? lp_rank<64>(v, i, count) : lane;             // in the tile's list
+                    if (__any(t.v != -INFINITY)) {
+                        wv[lane] = t.v;
+                        wi[lane] = t.i = t.i < LP_NONE ? t.i : LP_NONE + lane;
+                        lp_wave_sync();
+                        rank += lp_search(wv, wi, 64, v, i);                       // in both
+                        lp_wave_sync();
+                        const int mine = some ? rank : 64;                         // my column's place; the list's own entries move
+                        wv[lane] = -INFINITY;                                      // behind those of the tile that come before them
+                        wi[lane] = LP_NONE + lane;
+                        lp_wave_sync();
+                        int before = 0;
+                        for (int k = 0; k < count; k++) {
+                            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k));
+                            const int j = __builtin_amdgcn_readlane(i, k);
+                            before += lp_before(w, j, t.v, t.i);
+                        }
+                        if (lane + before < 64) {
+                            wv[lane + before] = t.v;
+                            wi[lane + before] = t.i;
+                        }
+                        rank = mine;
+                    }
+                    if (rank < 64) {
+                        wv[rank] = v;
+                        wi[rank] = i;
+                    }
+                    lp_wave_sync();
+                    t.v = wv[lane];
+                    t.i = wi[lane];
+                    lp_wave_sync();
                 }
                 worst = __shfl(t.v, A.top - 1);
             }
         }
-        s = lp_wave_join(s, A.c2);
-        __syncthreads();                                   // all waves' first tiles are done with the LDS arrays
-        if (lane == 0) lds_s[wave] = LpPart{ s.m, s.l, s.e, 0.0f };
-        if (TOP && lane < A.top) {
-            lds_v[wave * A.top + lane] = t.v;
-            lds_i[wave * A.top + lane] = t.i;
+    }
+    s = lp_wave_join(s, A.c2);
+    __syncthreads();                                   // all waves' first tiles are done with the LDS arrays
+    if (lane == 0) lds_s[wave] = LpPart{ s.m, s.l, s.e, 0.0f };
+    if (TOP && lane < A.top) {
+        lds_v[wave * A.top + lane] = t.v;
+        lds_i[wave * A.top + lane] = t.i = t.i < LP_NONE ? t.i : LP_NONE + (int)threadIdx.x;     // (no two entries the same)
+    }
+    __syncthreads();
+    s = LpStat();
+    if (lane < 4) {
+        s.m = lds_s[lane].m;
+        s.l = lds_s[lane].l;
+        s.e = lds_s[lane].e;
+    }
+    s = lp_wave_join(s, A.c2);
+    const float logl = logf(s.l);
+    if (threadIdx.x == 0) {
+        if (splits == 1) lp_write_row(A, row, s, logl, given);
+        else parts[unit] = LpPart{ s.m, s.l, s.e, 0.0f };
+    }
+    // the four lists together: an entry's place is its place in its own and the numbers of the others' entries before it
+    if (TOP && lane < A.top) {
+        int rank = lane;
+#pragma unroll
+        for (int k = 1; k < 4; k++) {
+            const int w = (wave + k) & 3;
+            rank += lp_search(lds_v + w * A.top, lds_i + w * A.top, A.top, t.v, t.i);
         }
-        __syncthreads();
-        if (wave == 0) {
-            s = LpStat();
-            if (lane < 4) {
-                s.m = lds_s[lane].m;
-                s.l = lds_s[lane].l;
-                s.e = lds_s[lane].e;
-            }
-            s = lp_wave_join(s, A.c2);
-            if constexpr (TOP) t = lp_merge(lds_v, lds_i, 4, A.top, lane);
-            if (splits == 1) {
-                const float logl = logf(s.l);
-                if (lane == 0) lp_write_row<E>(A, row, s, logl);
-                if (TOP && lane < A.top) lp_write_top(A, row, lane, t.v, t.i, s, logl);
-            } else {
-                if (lane == 0) parts[unit] = LpPart{ s.m, s.l, s.e, 0.0f };
-                if (TOP && lane < A.top) {
-                    part_v[unit * A.top + lane] = t.v;
-                    part_i[unit * A.top + lane] = t.i;
-                }
+        if (rank < A.top) {
+            if (splits == 1) lp_write_top(A, row, rank, t.v, t.i, s, logl);
+            else {
+                part_v[unit * A.top + rank] = t.v;
+                part_i[unit * A.top + rank] = t.i;
             }
         }
-        __syncthreads();                                   // the next unit's first tiles write the LDS arrays
     }
 }
 
-// the segments of a row together: one wavefront per row
+// The segments of a row together: one workgroup per row.  The lists come to LDS; of every list's entry number j (j as small as
+// `top` entries allow) the r-th largest is reached by `top` entries or more, few of them in general: they are the beginnings of their
+// lists, and are ranked as a short row's candidates are.  Where more than 64 are left, entry by entry (lp_merge).
 template <int E, bool TOP>
-__global__ __launch_bounds__(64) void k_logprobs_join(LpArgs A, int splits, const LpPart* __restrict__ parts, const float* __restrict__ part_v,
-                                                      const int* __restrict__ part_i)
+__global__ __launch_bounds__(256) void k_logprobs_join(LpArgs A, int splits, const LpPart* __restrict__ parts, const float* __restrict__ part_v,
+                                                       const int* __restrict__ part_i)
 {
+    __shared__ float lds_v[TOP ? LP_SPLITS * LP_TOP : 1], cand_v[TOP ? 64 : 1];
+    __shared__ int lds_i[TOP ? LP_SPLITS * LP_TOP : 1], cand_i[TOP ? 64 : 1];
     const long row = blockIdx.x;
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & 63, top = A.top;
+    if constexpr (TOP) {
+        for (int k = threadIdx.x; k < splits * top; k += 256) {
+            lds_v[k] = part_v[row * splits * top + k];
+            const int i = part_i[row * splits * top + k];
+            lds_i[k] = i < LP_NONE ? i : LP_NONE + k;
+        }
+    }
     LpStat s;
     if (lane < splits) {
         const LpPart q = parts[row * splits + lane];
@@ -549,12 +647,32 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LpArgs A, int splits, cons
         s.l = q.l;
         s.e = q.e;
     }
+    const float given = lp_given<E>(A, row);
     s = lp_wave_join(s, A.c2);
     const float logl = logf(s.l);
-    if (lane == 0) lp_write_row<E>(A, row, s, logl);
+    if (threadIdx.x == 0) lp_write_row(A, row, s, logl, given);
     if constexpr (TOP) {
-        const LpList t = lp_merge(part_v + row * splits * A.top, part_i + row * splits * A.top, splits, A.top, lane);
-        if (lane < A.top) lp_write_top(A, row, lane, t.v, t.i, s, logl);
+        __syncthreads();
+        if (threadIdx.x >= 64) return;
+        const int j = (top - 1) / splits, r = (top + j) / (j + 1);             // r lists with j + 1 entries each: r <= splits
+        const float T = lp_threshold<64>(lane < splits ? lds_v[lane * top + j] : -INFINITY, r, lane);
+        int mine = lane < splits ? lp_search(lds_v + lane * top, lds_i + lane * top, top, T, LP_NONE) : 0;      // this list's entries >= T
+        const int at = lp_before_me<64>(mine, lane), count = __builtin_amdgcn_readlane(at + mine, 63);
+        if (count <= 64) {
+            for (int k = 0; k < mine; k++) {
+                cand_v[at + k] = lds_v[lane * top + k];
+                cand_i[at + k] = lds_i[lane * top + k];
+            }
+            lp_wave_sync();
+            const float v = lane < count ? cand_v[lane] : -INFINITY;
+            const int i = lane < count ? cand_i[lane] : LP_NONE + lane;
+            int rank = lp_rank<64>(v, i, count);
+            if (lane >= count) rank = lane;
+            if (rank < top) lp_write_top(A, row, rank, v, i, s, logl);
+        } else {
+            const LpList t = lp_merge(lds_v, lds_i, splits, top, lane);
+            if (lane < top) lp_write_top(A, row, lane, t.v, t.i, s, logl);
+        }
     }
 }
 
@@ -612,13 +730,13 @@ static LpFactor lp_factor(double c)
 
 constexpr int LP_SHORT = 1024;                      // longest row that stays in a wavefront's registers
 
-// Segments of a long row: enough of them that the rows' fill the GPU, none shorter than four tiles
-static int lp_splits(int64_t rows, int cols)
+// Segments of a long row: enough of them that the rows' fill the GPU; a segment is a multiple of four tiles, one for each wavefront
+static int lp_segment(int64_t rows, int cols)
 {
-    if (cols <= LP_SHORT) return 1;
-    const int64_t want = (512 + rows - 1) / rows, most = std::max(1, cols / (4 * LP_TILE));
-    return (int)std::min<int64_t>({ want, most, LP_SPLITS });
+    const int64_t want = std::min<int64_t>((512 + rows - 1) / rows, LP_SPLITS), unit = 4 * LP_TILE;
+    return (int)(((cols + want - 1) / want + unit - 1) / unit * unit);
 }
+static int lp_splits(int64_t rows, int cols) { return cols <= LP_SHORT ? 1 : (cols - 1) / lp_segment(rows, cols) + 1; }
 
 int64_t action_logprobs_workspace(int64_t rows, int cols, int top)
 {
@@ -628,14 +746,12 @@ int64_t action_logprobs_workspace(int64_t rows, int cols, int top)
 
 constexpr long LP_GRID = 1 << 22;                   // workgroups per launch
 
-template <int E, int L, int V, int NV, int FULL> static void lp_launch_short(LpArgs A, hipStream_t st)
+// f(arguments of some rows), at most `most` rows at a time
+template <int E, class F> static void lp_chunks(LpArgs A, long most, F&& f)
 {
-    const long per = 256 / L, all = A.rows;
-    for (long row = 0; row < all; row += LP_GRID * per) {
-        A.rows = std::min(all - row, LP_GRID * per);
-        const unsigned grid = (unsigned)((A.rows + per - 1) / per);
-        if (A.top) k_logprobs_short<E, L, V, NV, FULL, true><<<grid, 256, 0, st>>>(A);
-        else k_logprobs_short<E, L, V, NV, FULL, false><<<grid, 256, 0, st>>>(A);
+    for (long left = A.rows; left > 0; left -= A.rows) {
+        A.rows = std::min(left, most);
+        f(A);
         A.x = (const char*)A.x + A.rows * A.xstride * (long)sizeof(typename Elem<E>::raw);
         if (A.valid) A.valid += A.rows * A.vstride;
         if (A.actions) A.actions += A.rows;
@@ -647,6 +763,16 @@ template <int E, int L, int V, int NV, int FULL> static void lp_launch_short(LpA
             A.top_logp += A.rows * A.top;
         }
     }
+}
+
+template <int E, int L, int V, int NV, int FULL> static void lp_launch_short(const LpArgs& all, hipStream_t st)
+{
+    const long per = 256 / L;
+    lp_chunks<E>(all, LP_GRID * per, [&](const LpArgs& A) {
+        const unsigned grid = (unsigned)((A.rows + per - 1) / per);
+        if (A.top) k_logprobs_short<E, L, V, NV, FULL, true><<<grid, 256, 0, st>>>(A);
+        else k_logprobs_short<E, L, V, NV, FULL, false><<<grid, 256, 0, st>>>(A);
+    });
 }
 
 template <int E> static void lp_launch(const LpArgs& A, void* workspace, hipStream_t st)
@@ -664,17 +790,19 @@ template <int E> static void lp_launch(const LpArgs& A, void* workspace, hipStre
         else if (A.cols <= 384) lp_launch_short<E, 64, 1, 6, 2>(A, st);
         else lp_launch_short<E, 64, 1, 16, 6>(A, st);
     } else {
-        const int splits = lp_splits(A.rows, A.cols);
-        const int segment = ((A.cols + splits - 1) / splits + LP_TILE - 1) / LP_TILE * LP_TILE;
+        const int segment = lp_segment(A.rows, A.cols), splits = lp_splits(A.rows, A.cols);
         LpPart* parts = (LpPart*)workspace;
         float* pv = (float*)(parts + A.rows * splits);
         int* pi = (int*)(pv + A.rows * splits * A.top);
-        const unsigned grid = (unsigned)std::min<long>(A.rows * splits, 1 << 20);
-        if (A.top) k_logprobs_long<E, true><<<grid, 256, 0, st>>>(A, splits, segment, parts, pv, pi);
-        else k_logprobs_long<E, false><<<grid, 256, 0, st>>>(A, splits, segment, parts, pv, pi);
+        // (splits > 1 only for fewer than 512 rows: one round)
+        lp_chunks<E>(A, LP_GRID, [&](const LpArgs& B) {
+            const unsigned grid = (unsigned)(B.rows * splits);
+            if (B.top) k_logprobs_long<E, true><<<grid, 256, 0, st>>>(B, splits, segment, parts, pv, pi);
+            else k_logprobs_long<E, false><<<grid, 256, 0, st>>>(B, splits, segment, parts, pv, pi);
+        });
         if (splits == 1) return;
-        if (A.top) k_logprobs_join<E, true><<<(unsigned)A.rows, 64, 0, st>>>(A, splits, parts, pv, pi);
-        else k_logprobs_join<E, false><<<(unsigned)A.rows, 64, 0, st>>>(A, splits, parts, pv, pi);
+        if (A.top) k_logprobs_join<E, true><<<(unsigned)A.rows, 256, 0, st>>>(A, splits, parts, pv, pi);
+        else k_logprobs_join<E, false><<<(unsigned)A.rows, 256, 0, st>>>(A, splits, parts, pv, pi);
     }
 }
 
