@@ -74,16 +74,22 @@ namespace goai {
 // four neighbouring elements from i on, as floats (zeros from `n` on); tensors are aligned to their element type only
 template <int E> __device__ __forceinline__ void aw_load(const void* base, long i, long n, float (&out)[4])
 {
-    using raw = typename Elem<E>::raw;
-    const raw* q = (const raw*)base + i;
-    for (int k = 0; k < 4; k++) out[k] = i + k < n ? elem_to_float<E>(q[k]) : 0.0f;
+    const typename Elem<E>::raw* q = (const typename Elem<E>::raw*)base + i;
+    if (i + 4 <= n) elem_load<E, 4>(q, out);
+    else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) out[k] = i + k < n ? elem_to_float<E>(q[k]) : 0.0f;
+    }
 }
 template <int E> __device__ __forceinline__ void aw_store(void* base, long i, long n, const float (&x)[4])
 {
-    using raw = typename Elem<E>::raw;
-    raw* q = (raw*)base + i;
-    for (int k = 0; k < 4; k++)
-        if (i + k < n) q[k] = elem_from_float<E>(x[k]);
+    typename Elem<E>::raw* q = (typename Elem<E>::raw*)base + i;
+    if (i + 4 <= n) elem_store<E, 4>(q, x);
+    else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (i + k < n) q[k] = elem_from_float<E>(x[k]);
+    }
 }
 
 __device__ __forceinline__ float aw_wave_max(float x)

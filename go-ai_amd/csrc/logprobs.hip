@@ -160,27 +160,47 @@ template <int L> __device__ __forceinline__ int lp_count(int n)
 // floats as integers of the same order, and back
 __device__ __forceinline__ int lp_key(int bits) { return bits ^ ((bits >> 31) & 0x7fffffff); }
 
-// The candidates of a group of L lanes for its `top` best columns: at least `top` of them (all, if there are fewer), bits as in
-// lp_at_least, `count` in the group; at most L unless several columns share the top-th value.
-// The first threshold, lp_threshold, is sharp while a lane seldom holds two of the best; where it leaves more than L, halving
-// the range between it and the largest value does (3.5 % of the wavefronts for 8 of 362 columns over 16 lanes, some 3 steps).
-template <int L, int N> __device__ __forceinline__ unsigned lp_candidates(const float (&x)[N], float lane_max, float most, int top, int lane, int& count)
+// The candidates of a group of L lanes for its `top` best columns: at least `top` of them (all, if there are fewer), at most L;
+// bits as in lp_at_least, `count` in the group.  Lane l holds vectors of V neighbouring columns, l V + q L V ...
+// The first threshold, lp_threshold, is sharp while a lane seldom holds two of the best.  Where it leaves more than L, the range
+// between it and the largest value is halved until it does not (3.5 % of the wavefronts for 8 of 362 columns over 16 lanes, some 3
+// steps), and where that ends at one value that too many columns share, the range of columns that count among them.
+template <int L, int V, int N> __device__ __forceinline__ unsigned lp_candidates(const float (&x)[N], float lane_max, float most, int top, int lane, int& count)
 {
     const float T = lp_threshold<L>(lane_max, top, lane);
     unsigned bits = lp_at_least(x, T);
     count = lp_count<L>(__popc(bits));
     if (__any(count > L)) {
         int lo = lp_key(__float_as_int(T)), hi = lp_key(__float_as_int(most)) + 1;       // enough columns reach lo, too few reach hi
-        for (int step = 0; step < 32 && __any(count > L && hi - lo > 1); step++) {
+        unsigned above = 0;                                                              // those that reach hi
+        while (__any(count > L && (unsigned)hi - (unsigned)lo > 1u)) {
             const int mid = (int)((unsigned)lo + (((unsigned)hi - (unsigned)lo) >> 1));
             const unsigned b = lp_at_least(x, __int_as_float(lp_key(mid)));
             const int n = lp_count<L>(__popc(b));
-            if (count > L) {
+            if (count > L && (unsigned)hi - (unsigned)lo > 1u) {
                 if (n >= top) {
                     lo = mid;
                     bits = b;
                     count = n;
-                } else hi = mid;
+                } else {
+                    hi = mid;
+                    above = b;
+                }
+            }
+        }
+        int c0 = 0, c1 = N * L;                              // too few, enough with the first so many columns of those at lo
+        const unsigned ties = bits & ~above;
+        const bool tied = count > L;
+        while (__any(count > L && c1 - c0 > 1)) {
+            const int mid = (c0 + c1) >> 1, q = mid / (L * V), mine = q * V + min(max(mid - (q * L + (lane & (L - 1))) * V, 0), V);
+            const unsigned b = above | (ties & (mine ? ~0u << (N - mine) : 0u));
+            const int n = lp_count<L>(__popc(b));
+            if (tied && count > L) {
+                if (n >= top) {
+                    c1 = mid;
+                    bits = b;
+                    count = n;
+                } else c0 = mid;
             }
         }
     }
@@ -299,8 +319,7 @@ __device__ __forceinline__ void lp_write_top(const LpArgs& A, long row, int rank
 //
 // The alternatives: T = lp_threshold of the lanes' maxima leaves few candidates (for 8 of 362 columns about 11).  The row goes to
 // LDS, every lane looks up its candidates there (a bit each), one lane takes each, and a candidate's place is the number of those
-// before it.  Where more than L remain (ties, masks that leave few columns to few lanes) the search is place by place: round r takes
-// the best column behind round r - 1's.
+// before it.
 
 template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs A)
 {
@@ -360,54 +379,28 @@ template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_b
 #pragma unroll
         for (int k = 0; k < N; k++) mine_x[k] = x[k];
         int count;
-        unsigned bits = lp_candidates<L>(x, lane_max, s.m, A.top, lane, count);
+        unsigned bits = lp_candidates<L, V>(x, lane_max, s.m, A.top, lane, count);
         int at = group + lp_before_me<L>(__popc(bits), sub);
         lp_wave_sync();
-        if (!__any(count > L)) {
-            while (__any(bits != 0)) {
-                if (bits) {
-                    const int k = __clz(bits) - (32 - N);
-                    bits &= ~(0x80000000u >> __clz(bits));
-                    lds_v[at] = mine_x[k];
-                    lds_i[at++] = min(((k / V) * L + sub) * V, last) + k % V;
-                }
-            }
-            lp_wave_sync();
-            const bool some = sub < count;
-            const float v = some ? lds_v[group + sub] : -INFINITY;
-            const int i = some ? lds_i[group + sub] : LP_NONE + sub;
-            int rank = lp_rank<L>(v, i, L == 64 ? count : L);
-            if (L == 64 && !some) rank = sub;                // behind all candidates
-            if (active && rank < A.top) lp_write_top(A, row, rank, v, i, s, logl);
-        } else {
-            float pv = INFINITY;                             // the place before
-            int pi = -1;
-            for (int r = 0; r < A.top; r++) {
-                float v = -INFINITY;
-                int i = LP_NONE;
-#pragma nounroll
-                for (int k = 0; k < N; k++) {
-                    const float w = mine_x[k];
-                    const int c = min(((k / V) * L + sub) * V, last) + k % V;
-                    if (w != -INFINITY && lp_before(pv, pi, w, c) && lp_before(w, c, v, i)) {
-                        v = w;
-                        i = c;
-                    }
-                }
-                for (int d = 1; d < L; d <<= 1) {
-                    const float w = __shfl_xor(v, d);
-                    const int j = __shfl_xor(i, d);
-                    if (lp_before(w, j, v, i)) { v = w; i = j; }
-                }
-                if (sub == 0 && active) lp_write_top(A, row, r, v, i, s, logl);
-                pv = v;
-                pi = i;
+        while (__any(bits != 0)) {
+            if (bits) {
+                const int k = __clz(bits) - (32 - N);
+                bits &= ~(0x80000000u >> __clz(bits));
+                lds_v[at] = mine_x[k];
+                lds_i[at++] = min(((k / V) * L + sub) * V, last) + k % V;
             }
         }
+        lp_wave_sync();
+        const bool some = sub < count;
+        const float v = some ? lds_v[group + sub] : -INFINITY;
+        const int i = some ? lds_i[group + sub] : LP_NONE + sub;
+        int rank = lp_rank<L>(v, i, L == 64 ? count : L);
+        if (L == 64 && !some) rank = sub;                // behind all candidates
+        if (active && rank < A.top) lp_write_top(A, row, rank, v, i, s, logl);
     }
 }
 
-// ---- long rows: a workgroup takes a segment of a row, each wavefront every fourth tile of it ----
+// ---- long rows: W wavefronts take a segment of a row, each of them every W-th tile of it ----
 //
 // A wavefront keeps its list of alternatives across its lanes.  A tile's columns come after all earlier tiles', so only those
 // strictly better than the last alternative listed can enter (k ln(n / k) of n, in random order): a few one by one, many -- the first
@@ -459,9 +452,10 @@ __device__ __forceinline__ int lp_search(const float* lv, const int* li, int top
     return at;
 }
 
-template <int E, bool TOP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k_logprobs_long(LpArgs A, int splits, int segment, LpPart* __restrict__ parts, float* __restrict__ part_v,
-                                                       int* __restrict__ part_i)
+template <int E, int W, bool TOP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k_logprobs_long(LpArgs A, int splits, int segment,
+                                                                                              LpPart* __restrict__ parts,
+                                                                                              float* __restrict__ part_v, int* __restrict__ part_i)
 {
     using raw = typename Elem<E>::raw;
     constexpr int V = E == 0 ? 4 : 8, NV = LP_E / V;
@@ -469,41 +463,42 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
     __shared__ int lds_i[TOP ? 256 : 1];
     __shared__ LpPart lds_s[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long unit = blockIdx.x;
-    const long row = unit / splits;
-    const int split = (int)(unit - row * splits);
+    const long unit = W == 4 ? (long)blockIdx.x : (long)blockIdx.x * 4 + wave;
+    if (W == 1 && unit >= A.rows) return;
+    const long row = W == 4 ? unit / splits : unit;
+    const int split = W == 4 ? (int)(unit - row * splits) : 0;
     const int c0 = split * segment, c1 = min(A.cols, c0 + segment);
     const raw* p = (const raw*)A.x + row * A.xstride;
     const uint8_t* valid = A.valid ? A.valid + row * A.vstride : nullptr;
     const float given = splits == 1 ? lp_given<E>(A, row) : 0.0f;
     LpStat s;
     LpList t;
-    float worst = -INFINITY;                           // the last alternative of the tiles before
-    for (int base = c0 + wave * LP_TILE; base < c1; base += 4 * LP_TILE) {
+    float worst = -INFINITY;                               // the last alternative of the tiles before
+    for (int base = c0 + (W == 4 ? wave : 0) * LP_TILE; base < c1; base += W * LP_TILE) {
+        // the loads are issued before the first is used; a vector that would pass the row's end starts V columns before it, and its
+        // columns in front of the lane's own are another lane's (rows of this kernel are longer than a tile)
         float x[LP_E];
-        if (base + LP_TILE <= c1) {
+        {
+            ElemVec<E, V> u[NV];
+            const int last = A.cols - V;
 #pragma unroll
-            for (int q = 0; q < NV; q++) {
-                const int c = base + (q * 64 + lane) * V;
-                float u[V];
-                elem_load<E, V>(p + c, u);
-#pragma unroll
-                for (int k = 0; k < V; k++) x[q * V + k] = u[k];
-            }
+            for (int q = 0; q < NV; q++) __builtin_memcpy(&u[q], p + min(base + (q * 64 + lane) * V, last), sizeof(u[q]));
             if (valid) {
+                uint8_t ok[NV][V];
 #pragma unroll
-                for (int q = 0; q < NV; q++) {
-                    uint8_t ok[V];
-                    __builtin_memcpy(ok, valid + base + (q * 64 + lane) * V, V);
+                for (int q = 0; q < NV; q++) __builtin_memcpy(ok[q], valid + min(base + (q * 64 + lane) * V, last), V);
 #pragma unroll
-                    for (int k = 0; k < V; k++) x[q * V + k] = ok[k] ? x[q * V + k] : -INFINITY;
-                }
+                for (int k = 0; k < LP_E; k++) x[k] = ok[k / V][k % V] ? elem_to_float<E>(u[k / V].a[k % V]) : -INFINITY;
+            } else {
+#pragma unroll
+                for (int k = 0; k < LP_E; k++) x[k] = elem_to_float<E>(u[k / V].a[k % V]);
             }
-        } else {
+            if (base + LP_TILE > A.cols) {
 #pragma unroll
-            for (int k = 0; k < LP_E; k++) {
-                const int c = base + ((k / V) * 64 + lane) * V + k % V;
-                x[k] = c < c1 && (!valid || valid[c]) ? elem_to_float<E>(p[c]) : -INFINITY;
+                for (int k = 0; k < LP_E; k++) {
+                    const int c = base + ((k / V) * 64 + lane) * V;
+                    x[k] = min(c, last) + k % V >= c ? x[k] : -INFINITY;
+                }
             }
         }
         float lane_max = -INFINITY;
@@ -514,34 +509,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
         for (int k = 0; k < LP_E; k++) lp_add(s, x[k], A.c2);
         if constexpr (TOP) {
             if (__any(lane_max > worst)) {
-                unsigned enter = 0xffffffffu;              // columns that may enter, if above the last one listed
-                int count = 0;
+                const int last = A.cols - V;
                 // more than a few: the tile's own list, by threshold and rank as a short row's, and the two lists merged
-                bool one_by_one = lp_count<64>(__popc(lp_at_least(x, fmaxf(worst, -FLT_MAX)))) <= LP_FEW;
-                if (!one_by_one) {
-                    enter = lp_candidates<64>(x, lane_max, lp_max<64>(lane_max), A.top, lane, count);
-                    one_by_one = count > 64;               // (ties)
-                }
-                if (one_by_one) {
+                if (lp_count<64>(__popc(lp_at_least(x, fmaxf(worst, -FLT_MAX)))) <= LP_FEW) {
+                    const float bar = worst;
 #pragma unroll
                     for (int k = 0; k < LP_E; k++) {
-                        if (k && k % V == 0) worst = __shfl(t.v, A.top - 1);       // the next vectors' columns come after these
-                        unsigned long long better = __ballot(x[k] > worst && (enter & (1u << (LP_E - 1 - k))));
+                        unsigned long long better = __ballot(x[k] > bar);
                         while (better) {
                             const int src = __ffsll((long long)better) - 1;
                             better &= better - 1;
-                            lp_insert(t, __shfl(x[k], src), base + ((k / V) * 64 + src) * V + k % V, lane);
+                            lp_insert(t, __shfl(x[k], src), min(base + ((k / V) * 64 + src) * V, last) + k % V, lane);
                         }
                     }
                 } else {
                     float* wv = lds_v + wave * 64;
                     int* wi = lds_i + wave * 64;
+                    int count;
+                    const unsigned enter = lp_candidates<64, V>(x, lane_max, lp_max<64>(lane_max), A.top, lane, count);
                     int at = lp_before_me<64>(__popc(enter), lane);
 #pragma unroll
                     for (int k = 0; k < LP_E; k++)
                         if (enter & (1u << (LP_E - 1 - k))) {
                             wv[at] = x[k];
-                            wi[at++] = base + ((k / V) * 64 + lane) * V + k % V;
+                            wi[at++] = min(base + ((k / V) * 64 + lane) * V, last) + k % V;
                         }
                     lp_wave_sync();
                     const bool some = lane < count;
@@ -585,6 +576,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
         }
     }
     s = lp_wave_join(s, A.c2);
+    if constexpr (W == 1) {
+        const float logl = logf(s.l);
+        if (lane == 0) lp_write_row(A, row, s, logl, given);
+        if (TOP && lane < A.top) lp_write_top(A, row, lane, t.v, t.i, s, logl);
+        return;
+    }
     __syncthreads();                                   // all waves' first tiles are done with the LDS arrays
     if (lane == 0) lds_s[wave] = LpPart{ s.m, s.l, s.e, 0.0f };
     if (TOP && lane < A.top) {
@@ -690,27 +687,63 @@ struct LpGradArgs {
     int cols;
 };
 
-template <int E> __device__ __forceinline__ float lp_grad_of(float x, bool ok, bool hot, float inv_t, float lse, float H, float g, float h)
-{
-    if (!ok || x == -INFINITY) return 0.0f;
-    const float lp = __builtin_amdgcn_fmed3f(x * inv_t, -FLT_MAX, FLT_MAX) - lse, p = __builtin_amdgcn_exp2f(lp * LOG2E);
-    const float pl = p > 0.0f ? p * (lp + H) : (p == 0.0f ? 0.0f : p);        // (NaN stays)
-    return ((hot ? g : 0.0f) - g * p - h * pl) * inv_t;
-}
+// One pass: L lanes a row, up to LG_N vectors of V columns each; L = 256: workgroups (row, chunk of a long row).  Bound by reading the
+// logits and the mask and writing the gradient.  The logits may be the output: a lane writes the columns that it alone reads.
+constexpr int LG_N = 4;
 
-template <int E> __global__ __launch_bounds__(256) void k_logprobs_grad(LpGradArgs A)
+template <int E, int L, int V> __global__ __launch_bounds__(256) void k_logprobs_grad(LpGradArgs A, int chunks)
 {
     using raw = typename Elem<E>::raw;
-    const int lane = threadIdx.x & 63;
-    for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < A.rows; row += (long)gridDim.x * 4) {
+    const int sub = threadIdx.x & (L - 1);
+    long row;
+    int c0 = 0;
+    if constexpr (L == 256) {
+        row = blockIdx.x / chunks;
+        c0 = (int)(blockIdx.x - row * chunks) * (LG_N * L * V);
+    } else {
+        row = (long)blockIdx.x * (256 / L) + threadIdx.x / L;
+        if (row >= A.rows) return;
+    }
     const raw* x = (const raw*)A.x + row * A.xstride;
     raw* dx = (raw*)A.dx + row * A.dstride;
-    const uint8_t* valid = A.valid ? A.valid + row * A.vstride : nullptr;
+    // a vector that would pass the row's end is read from V columns before it (cols >= V)
+    const int last = A.cols - V;
+    ElemVec<E, V> u[LG_N];
+#pragma unroll
+    for (int q = 0; q < LG_N; q++)
+        if (c0 + q * L * V < A.cols) __builtin_memcpy(&u[q], x + min(c0 + (q * L + sub) * V, last), sizeof(u[q]));
+    uint8_t ok[LG_N][V];
+    if (A.valid) {
+        const uint8_t* valid = A.valid + row * A.vstride;
+#pragma unroll
+        for (int q = 0; q < LG_N; q++)
+            if (c0 + q * L * V < A.cols) __builtin_memcpy(ok[q], valid + min(c0 + (q * L + sub) * V, last), V);
+    } else {
+#pragma unroll
+        for (int k = 0; k < LG_N * V; k++) ok[k / V][k % V] = 1;
+    }
     const int a = A.actions ? A.actions[row] : -1;
     const float lse = A.lse[row], H = A.h ? A.entropy[row] : 0.0f, h = A.h ? A.h[row] : 0.0f;
     const float g = a < 0 ? 0.0f : a >= A.cols ? NAN : A.g[row];
-    for (int c = lane; c < A.cols; c += 64)
-        dx[c] = elem_from_float<E>(lp_grad_of<E>(elem_to_float<E>(x[c]), !valid || valid[c], c == a, A.inv_t, lse, H, g, h));
+#pragma unroll
+    for (int q = 0; q < LG_N; q++) {
+        const int c = c0 + (q * L + sub) * V, cc = min(c, last);
+        if (c >= A.cols) break;
+        float d[V];
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const float v = elem_to_float<E>(u[q].a[k]);
+            const float lp = __builtin_amdgcn_fmed3f(v * A.inv_t, -FLT_MAX, FLT_MAX) - lse, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+            // p log p is 0 at p = 0, also where log p is -inf
+            const float t = fmaf(h, p * fmaxf(lp + H, -1000.0f), g * p);
+            d[k] = ok[q][k] && v != -INFINITY ? ((cc + k == a ? g : 0.0f) - t) * A.inv_t : 0.0f;
+        }
+        if (c == cc) elem_store<E, V>(dx + c, d);
+        else {
+#pragma unroll
+            for (int k = 0; k < V; k++)
+                if (cc + k >= c) dx[cc + k] = elem_from_float<E>(d[k]);
+        }
     }
 }
 
@@ -730,7 +763,10 @@ static LpFactor lp_factor(double c)
 
 constexpr int LP_SHORT = 1024;                      // longest row that stays in a wavefront's registers
 
-// Segments of a long row: enough of them that the rows' fill the GPU; a segment is a multiple of four tiles, one for each wavefront
+// Long rows: from LP_MANY rows on they fill the GPU a wavefront each (20000 x 2000 float32, 5 alternatives: 40 us, with four wavefronts a
+// row 85; 2048 x 40000: 67 and 70; 1024 x 40000: 56 and 37); fewer rows take four wavefronts a segment, in as many segments as fill
+// it.  A segment is a multiple of four tiles, one for each.
+constexpr int64_t LP_MANY = 2048;
 static int lp_segment(int64_t rows, int cols)
 {
     const int64_t want = std::min<int64_t>((512 + rows - 1) / rows, LP_SPLITS), unit = 4 * LP_TILE;
@@ -795,10 +831,13 @@ template <int E> static void lp_launch(const LpArgs& A, void* workspace, hipStre
         float* pv = (float*)(parts + A.rows * splits);
         int* pi = (int*)(pv + A.rows * splits * A.top);
         // (splits > 1 only for fewer than 512 rows: one round)
+        const bool many = A.rows >= LP_MANY;
         lp_chunks<E>(A, LP_GRID, [&](const LpArgs& B) {
-            const unsigned grid = (unsigned)(B.rows * splits);
-            if (B.top) k_logprobs_long<E, true><<<grid, 256, 0, st>>>(B, splits, segment, parts, pv, pi);
-            else k_logprobs_long<E, false><<<grid, 256, 0, st>>>(B, splits, segment, parts, pv, pi);
+            const unsigned grid = many ? (unsigned)((B.rows + 3) / 4) : (unsigned)(B.rows * splits);
+            if (many && B.top) k_logprobs_long<E, 1, true><<<grid, 256, 0, st>>>(B, 1, B.cols, parts, pv, pi);
+            else if (many) k_logprobs_long<E, 1, false><<<grid, 256, 0, st>>>(B, 1, B.cols, parts, pv, pi);
+            else if (B.top) k_logprobs_long<E, 4, true><<<grid, 256, 0, st>>>(B, splits, segment, parts, pv, pi);
+            else k_logprobs_long<E, 4, false><<<grid, 256, 0, st>>>(B, splits, segment, parts, pv, pi);
         });
         if (splits == 1) return;
         if (A.top) k_logprobs_join<E, true><<<(unsigned)A.rows, 256, 0, st>>>(A, splits, parts, pv, pi);
@@ -817,13 +856,41 @@ int launch_action_logprobs(const void* logits, int elem, int64_t stride, const u
     return GOAI_OK;
 }
 
+template <int E, int L, int V> static void lp_launch_grad(LpGradArgs A, hipStream_t st)
+{
+    const int chunks = L == 256 ? (A.cols + LG_N * L * V - 1) / (LG_N * L * V) : 1;
+    const long most = std::max<long>(1, LP_GRID / chunks) * (256 / L);
+    for (long left = A.rows; left > 0; left -= A.rows) {
+        A.rows = std::min(left, most);
+        k_logprobs_grad<E, L, V><<<(unsigned)(L == 256 ? A.rows * chunks : (A.rows + 256 / L - 1) / (256 / L)), 256, 0, st>>>(A, chunks);
+        const long size = sizeof(typename Elem<E>::raw);
+        A.x = (const char*)A.x + A.rows * A.xstride * size;
+        A.dx = (char*)A.dx + A.rows * A.dstride * size;
+        if (A.valid) A.valid += A.rows * A.vstride;
+        if (A.actions) A.actions += A.rows;
+        A.lse += A.rows;
+        if (A.entropy) A.entropy += A.rows;
+        if (A.g) A.g += A.rows;
+        if (A.h) A.h += A.rows;
+    }
+}
+template <int E> static void lp_launch_grad(const LpGradArgs& A, hipStream_t st)
+{
+    constexpr int V = E == 0 ? 4 : 8;                   // 16 bytes; 8 of a short row, which has few vectors for its lanes (300000 x 26
+    if (A.cols < 4) lp_launch_grad<E, 16, 1>(A, st);    // bfloat16: TIMEC us, with 16 bytes 30)
+    else if (A.cols <= LG_N * 16 * 4) lp_launch_grad<E, 16, 4>(A, st);
+    else if (A.cols <= LG_N * 16 * V) lp_launch_grad<E, 16, V>(A, st);
+    else if (A.cols <= LG_N * 64 * V) lp_launch_grad<E, 64, V>(A, st);
+    else lp_launch_grad<E, 256, V>(A, st);
+}
+
 int launch_action_logprobs_grad(const void* logits, int elem, int64_t stride, const uint8_t* valid, int64_t valid_stride,
                                 const int32_t* actions, double temperature, const float* lse, const float* entropy, const float* d_logp,
                                 const float* d_entropy, void* d_logits, int64_t d_stride, int64_t rows, int cols, hipStream_t st)
 {
-    const LpGradArgs A{ logits, (long)stride, valid, (long)valid_stride, d_logp ? actions : nullptr, (float)(1.0 / temperature), lse, entropy, d_logp,
-                        d_entropy, d_logits, (long)d_stride, (long)rows, cols };
-    LP_DISPATCH(elem, k_logprobs_grad<E><<<(unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 20), 256, 0, st>>>(A));
+    LpGradArgs A{ logits, (long)stride, valid, (long)valid_stride, d_logp ? actions : nullptr, (float)(1.0 / temperature), lse, entropy, d_logp,
+                  d_entropy, d_logits, (long)d_stride, (long)rows, cols };
+    LP_DISPATCH(elem, lp_launch_grad<E>(A, st));
     GOAI_HIP_CHECK(hipGetLastError());
     return GOAI_OK;
 }

@@ -15,6 +15,9 @@ from . import _hip
 
 NUM_CHNLS = 6
 
+# the current stream's handle without a Stream object (0.1 instead of 1.9 us of every call), where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
 
 def _dev_u8_states(states, device):
     if isinstance(states, np.ndarray):
@@ -77,6 +80,8 @@ class Context:
         if self._h is None:
             raise RuntimeError("this go_ai.engine.Context was closed (evicted from a context cache, or close() was called): "
                                "its device state is gone")
+        if _raw_stream is not None and _raw_stream(self.device_index) == self._stream.cuda_stream:
+            return
         cur = torch.cuda.current_stream(self.device)
         if cur.cuda_stream != self._stream.cuda_stream:
             self._stream.synchronize()
@@ -205,8 +210,9 @@ class Context:
     def _per_row(self, x, rows, dtype, what):
         if x is None:
             return None
-        x = torch.as_tensor(x)
-        if x.dtype != dtype or x.device != self.device or not x.is_contiguous():
+        if not torch.is_tensor(x):
+            x = torch.as_tensor(x)
+        if x.dtype is not dtype or x.device != self.device or not x.is_contiguous():
             x = x.to(self.device, dtype=dtype).contiguous()
         if x.numel() != rows:
             raise ValueError(f"{what}: one number for each of the {rows} rows, got shape {tuple(x.shape)}")
@@ -227,12 +233,12 @@ class Context:
         top = int(top)
         if not 0 <= top <= self.LOGPROBS_MAX_TOP:
             raise ValueError(f"top must be in 0 .. {self.LOGPROBS_MAX_TOP}")
-        out = torch.empty((3, rows), dtype=torch.float32, device=self.device)
+        out = x.new_empty((3, rows), dtype=torch.float32)
         logp, entropy, lse = out.unbind(0)
         best = best_lp = None
         if top:
-            best = torch.empty((rows, top), dtype=torch.int32, device=self.device)
-            best_lp = torch.empty((rows, top), dtype=torch.float32, device=self.device)
+            best = x.new_empty((rows, top), dtype=torch.int32)
+            best_lp = x.new_empty((rows, top), dtype=torch.float32)
         if a is None:
             logp = None
         if rows:
@@ -255,7 +261,7 @@ class Context:
         l, e = self._per_row(lse, rows, torch.float32, "lse"), self._per_row(entropy, rows, torch.float32, "entropy")
         g, h = self._per_row(d_logp, rows, torch.float32, "d_logp"), self._per_row(d_entropy, rows, torch.float32, "d_entropy")
         if out is None:
-            out = torch.empty((rows, cols), dtype=x.dtype, device=self.device)
+            out = x.new_empty((rows, cols))
         elif (out.dtype != x.dtype or tuple(out.shape) != (rows, cols) or out.device != self.device
               or (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols)):
             raise ValueError("out: a matrix of the logits' shape, type and device, its columns next to each other")

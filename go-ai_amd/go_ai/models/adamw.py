@@ -126,14 +126,14 @@ class AdamW:
     def _grads(self, grads):
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW: {len(self.params)} parameters, {len(grads)} gradients")
-        table, device = self._table, self.device
+        table, device = self._table, self.device.index
         for i, (g, dtype, shape) in enumerate(zip(grads, self._gtypes, self._shapes)):
             if g is None:
                 table[i] = None
-            elif g.dtype is dtype and g.shape == shape and g.device == device and g.is_contiguous():
+            elif g.dtype is dtype and g.shape == shape and g.get_device() == device and g.is_contiguous():
                 table[i] = g.data_ptr()
             else:
-                raise ValueError(f"AdamW: gradient {i} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, got {g.dtype} "
+                raise ValueError(f"AdamW: gradient {i} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {self.device}, got {g.dtype} "
                                  f"of shape {tuple(g.shape)} on {g.device}, strides {g.stride()}")
         return table
 
