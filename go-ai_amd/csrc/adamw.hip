@@ -15,6 +15,7 @@
 //      fraction bits, the largest r of the block is 1.0 = code 255; half a step: 2^-5 of r), 0 for r = 0.  A root that is not zero
 //      never becomes 0: m / (0 + eps) would throw the parameter away.
 // The update itself uses the moments before they are rounded.  A block whose largest value is below 2^-100 is held as zeros.
+#include <float.h>
 #include <math.h>
 #include <string.h>
 
@@ -28,12 +29,12 @@
 
 namespace goai {
 
-constexpr int AW_BLOCK = 256;          // elements per scale of an 8-bit moment: four per lane of a wavefront
-constexpr int AW_CHUNK = 2048;         // elements per workgroup
+constexpr int AW_BLOCK = 256;          // elements per scale of an 8-bit moment: eight on each of 32 lanes
+constexpr int AW_CHUNK = 2048;         // elements per workgroup: eight per thread
 constexpr int AW_LEVEL0 = 1777;        // (255 + AW_LEVEL0) << 19 is 1.0f
 constexpr float AW_SMALLEST = 0x1p-100f;
 constexpr int AW_LAUNCH = 256;         // tensors per launch: their gradients' addresses travel in the launch's arguments
-constexpr int AW_NORM_BLOCKS = 1024;   // workgroups (and float64 partial sums) of the norm
+constexpr int AW_NORM_BLOCKS = 2048;   // workgroups (and float64 partial sums) of the norm
 
 struct AwTensor {
     void* p;
@@ -71,109 +72,203 @@ struct goai_adamw {
 
 namespace goai {
 
-// four neighbouring elements from i on, as floats (zeros from `n` on); tensors are aligned to their element type only
-template <int E> __device__ __forceinline__ void aw_load(const void* base, long i, long n, float (&out)[4])
+// N neighbouring elements from i on, as floats (zeros from `n` on); tensors are aligned to their element type only.  FULL: all of
+// them are inside for sure, and all loads of a thread are in flight together
+template <int E, bool FULL = false, int N> __device__ __forceinline__ void aw_load(const void* base, long i, long n, float (&out)[N])
 {
     const typename Elem<E>::raw* q = (const typename Elem<E>::raw*)base + i;
-    if (i + 4 <= n) elem_load<E, 4>(q, out);
+    if (FULL || i + N <= n) elem_load<E, N>(q, out);
     else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) out[k] = i + k < n ? elem_to_float<E>(q[k]) : 0.0f;
+        for (int k = 0; k < N; k++) out[k] = i + k < n ? elem_to_float<E>(q[k]) : 0.0f;
     }
 }
-template <int E> __device__ __forceinline__ void aw_store(void* base, long i, long n, const float (&x)[4])
+template <int E, bool FULL = false, int N> __device__ __forceinline__ void aw_store(void* base, long i, long n, const float (&x)[N])
 {
     typename Elem<E>::raw* q = (typename Elem<E>::raw*)base + i;
-    if (i + 4 <= n) elem_store<E, 4>(q, x);
+    if (FULL || i + N <= n) elem_store<E, N>(q, x);
     else {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < N; k++)
             if (i + k < n) q[k] = elem_from_float<E>(x[k]);
     }
 }
 
-__device__ __forceinline__ float aw_wave_max(float x)
+// The largest of 32 lanes' floats >= 0, which are ordered as their bits (a NaN above all).
+template <int CTRL> __device__ __forceinline__ unsigned aw_dpp(unsigned x) { return (unsigned)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true); }
+__device__ __forceinline__ float aw_max32(unsigned x)
 {
-    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
+    x = max(x, aw_dpp<0x128>(x));          // rotations within 16 lanes by 8, 4, 2, 1
+    x = max(x, aw_dpp<0x124>(x));
+    x = max(x, aw_dpp<0x122>(x));
+    x = max(x, aw_dpp<0x121>(x));
+    return __uint_as_float(max(x, (unsigned)__shfl_xor((int)x, 16)));
 }
 
-// ---- moments in 8 bits: four neighbouring codes per lane, a block per wavefront ----
-__device__ __forceinline__ void aw_mean_of(unsigned code, float scale, float (&m)[4])
+// Square roots, correctly rounded: y = 1 / sqrt(x) to an ulp, s = x y, and one correction s + (x - s s) y / 2.  Against sqrtf it gives
+// the same for every x from 2^-102 on (all of them compared); sqrtf's own correction steps take twice the instructions.
+// 0: y is held finite.  Smaller x, infinities and NaN: sqrtf.
+template <int N> __device__ __forceinline__ void aw_sqrt(const float (&x)[N], float (&s)[N])
 {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(code, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
-    m[0] = lo[0] * scale;
-    m[1] = lo[1] * scale;
-    m[2] = hi[0] * scale;
-    m[3] = hi[1] * scale;
+    unsigned least = 0xffffffffu, most = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const unsigned bits = __float_as_uint(x[k]);
+        least = min(least, bits - 1);      // 0 counts as the largest
+        most = max(most, bits);
+    }
+    if (__any(least < __float_as_uint(0x1p-100f) || most >= 0x7f800000u)) {
+#pragma unroll
+        for (int k = 0; k < N; k++) s[k] = sqrtf(x[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const float y = __builtin_amdgcn_fmed3f(__builtin_amdgcn_rsqf(x[k]), 0.0f, FLT_MAX), r = x[k] * y;
+            s[k] = fmaf(fmaf(-r, r, x[k]), y * 0.5f, r);
+        }
+    }
 }
-__device__ __forceinline__ void aw_root_of(unsigned code, float scale, float (&r)[4])
+
+// ---- moments in 8 bits: eight neighbouring codes per lane, a block on 32 lanes ----
+struct AwCodes {
+    unsigned w[2];
+};
+__device__ __forceinline__ void aw_mean_of(AwCodes code, float scale, float (&m)[8])
 {
-    for (int k = 0; k < 4; k++) {
-        const unsigned c = (code >> (8 * k)) & 255u;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(code.w[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(code.w[h], true);
+        m[4 * h] = lo[0] * scale;
+        m[4 * h + 1] = lo[1] * scale;
+        m[4 * h + 2] = hi[0] * scale;
+        m[4 * h + 3] = hi[1] * scale;
+    }
+}
+__device__ __forceinline__ void aw_root_of(AwCodes code, float scale, float (&r)[8])
+{
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const unsigned c = (code.w[k / 4] >> (8 * (k % 4))) & 255u;
         r[k] = c ? __uint_as_float((c + AW_LEVEL0) << 19) * scale : 0.0f;
     }
 }
-__device__ __forceinline__ unsigned aw_pack_mean(const float (&m)[4], float& scale)
+__device__ __forceinline__ AwCodes aw_pack_mean(const float (&m)[8], float& scale)
 {
-    const float big = aw_wave_max(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
+    unsigned most = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) most = max(most, __float_as_uint(m[k]) & 0x7fffffffu);
+    const float big = aw_max32(most);
     const bool held = big >= AW_SMALLEST;
     const float inv = held ? (1.0f / big) * 448.0f : 0.0f;
     scale = held ? big * (1.0f / 448.0f) : 0.0f;
-    int code = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * inv, m[1] * inv, 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(m[2] * inv, m[3] * inv, code, true);
+    AwCodes c;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(m[4 * h] * inv, m[4 * h + 1] * inv, 0, false);
+        c.w[h] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(m[4 * h + 2] * inv, m[4 * h + 3] * inv, lo, true);
+    }
+    return c;
 }
-__device__ __forceinline__ unsigned aw_pack_root(const float (&r)[4], float& scale)
+__device__ __forceinline__ AwCodes aw_pack_root(const float (&r)[8], float& scale)
 {
-    const float big = aw_wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
+    unsigned most = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) most = max(most, __float_as_uint(r[k]));
+    const float big = aw_max32(most);
     const bool held = big >= AW_SMALLEST;
     const float inv = held ? 1.0f / big : 0.0f;
     scale = held ? big : 0.0f;
-    unsigned code = 0;
-    for (int k = 0; k < 4; k++) {
-        const unsigned bits = __float_as_uint(r[k] * inv);
-        const int c = (int)((bits + 0x3FFFFu + ((bits >> 19) & 1u)) >> 19) - AW_LEVEL0;
-        code |= (held && r[k] > 0.0f ? (unsigned)min(max(c, 1), 255) : 0u) << (8 * k);
+    AwCodes code{ { 0, 0 } };
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        // to the nearest, ties to even, in units of the code; what is not zero is 1 at least (also where big is infinite)
+        const int bits = __float_as_int(r[k] * inv);
+        const int c = (bits + (int)(0x3FFFFu - ((unsigned)AW_LEVEL0 << 19)) + ((bits >> 19) & 1)) >> 19;
+        code.w[k / 4] |= (unsigned)min(max(c, (int)min(__float_as_uint(r[k]), 1u)), 255) << (8 * (k % 4));
     }
     return code;
 }
 
 // ---- the step ----
-template <int BITS, int PE, int GE>
-__device__ __forceinline__ void aw_update(const AwTensor& T, const AwState& S, const void* g_base, long i, int lane, const AwScal& s, float k, float keep)
+//
+// Bound by memory: 28 bytes an element in float32, 16 with moments in 8 bits, 10 with bfloat16 parameters and gradients too, at
+// some 55 vector instructions an element (39 T lane instructions a second: 1.4 ps, 10 bytes at 5 TB/s take 2).  The quotient is a
+// product with the reciprocal (an ulp or two of the update).
+template <int N>
+__device__ __forceinline__ void aw_math(float (&p)[N], const float (&g)[N], float (&m)[N], float (&v)[N], float (&root)[N], const AwScal& s, float k,
+                                        float keep)
 {
-    float p[4], g[4], m[4], v[4], root[4];
+#pragma unroll
+    for (int q = 0; q < N; q++) {
+        const float gk = g[q] * k;
+        m[q] = m[q] * s.b1 + gk * s.omb1;
+        v[q] = v[q] * s.b2 + gk * gk * s.omb2;
+    }
+    aw_sqrt(v, root);
+#pragma unroll
+    for (int q = 0; q < N; q++) p[q] = p[q] * keep - (m[q] * __builtin_amdgcn_rcpf(root[q] * s.c1 + s.eps)) * s.c2;
+}
+
+// eight elements of a tensor with 8-bit moments, from i on
+template <int PE, int GE, bool FULL>
+__device__ __forceinline__ void aw_update8(const AwTensor& T, const AwState& S, const void* g_base, long i, const AwScal& s, float k, float keep)
+{
+    float p[8], g[8], m[8], v[8], root[8];
     const long j = T.start + i;
-    aw_load<PE>(T.p, i, T.n, p);
-    aw_load<GE>(g_base, i, T.n, g);
-    if constexpr (BITS == 32) {
-        aw_load<0>((float*)S.m + T.start, i, T.n, m);
-        aw_load<0>((float*)S.v + T.start, i, T.n, v);
-    } else {
-        aw_mean_of(((const unsigned*)S.m)[j / 4], S.ms[j / AW_BLOCK], m);
-        aw_root_of(((const unsigned*)S.v)[j / 4], S.vs[j / AW_BLOCK], v);
-        for (int q = 0; q < 4; q++) v[q] = v[q] * v[q];
+    aw_load<PE, FULL>(T.p, i, T.n, p);
+    aw_load<GE, FULL>(g_base, i, T.n, g);
+    aw_mean_of(*(const AwCodes*)((const char*)S.m + j), S.ms[j / AW_BLOCK], m);
+    aw_root_of(*(const AwCodes*)((const char*)S.v + j), S.vs[j / AW_BLOCK], v);
+#pragma unroll
+    for (int q = 0; q < 8; q++) v[q] = v[q] * v[q];
+    aw_math(p, g, m, v, root, s, k, keep);
+    aw_store<PE, FULL>(T.p, i, T.n, p);
+    float ms, vs;
+    *(AwCodes*)((char*)S.m + j) = aw_pack_mean(m, ms);
+    *(AwCodes*)((char*)S.v + j) = aw_pack_root(root, vs);
+    if (j % AW_BLOCK == 0) {
+        S.ms[j / AW_BLOCK] = ms;
+        S.vs[j / AW_BLOCK] = vs;
     }
-    for (int q = 0; q < 4; q++) {
-        g[q] = g[q] * k;
-        m[q] = m[q] * s.b1 + g[q] * s.omb1;
-        v[q] = v[q] * s.b2 + g[q] * g[q] * s.omb2;
-        root[q] = sqrtf(v[q]);
-        p[q] = p[q] * keep - (m[q] / (root[q] * s.c1 + s.eps)) * s.c2;
+}
+
+// four elements of a tensor with 32-bit moments, from i and from i + 1024 on
+template <int PE, int GE, bool FULL>
+__device__ __forceinline__ void aw_update32(const AwTensor& T, const AwState& S, const void* g_base, long i, const AwScal& s, float k, float keep)
+{
+    float p[2][4], g[2][4], m[2][4], v[2][4], root[4];
+    float *mt = (float*)S.m + T.start, *vt = (float*)S.v + T.start;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        aw_load<PE, FULL>(T.p, i + 1024 * h, T.n, p[h]);
+        aw_load<GE, FULL>(g_base, i + 1024 * h, T.n, g[h]);
+        aw_load<0, FULL>(mt, i + 1024 * h, T.n, m[h]);
+        aw_load<0, FULL>(vt, i + 1024 * h, T.n, v[h]);
     }
-    aw_store<PE>(T.p, i, T.n, p);
-    if constexpr (BITS == 32) {
-        aw_store<0>((float*)S.m + T.start, i, T.n, m);
-        aw_store<0>((float*)S.v + T.start, i, T.n, v);
-    } else {
-        float ms, vs;
-        ((unsigned*)S.m)[j / 4] = aw_pack_mean(m, ms);
-        ((unsigned*)S.v)[j / 4] = aw_pack_root(root, vs);
-        if (lane == 0) {
-            S.ms[j / AW_BLOCK] = ms;
-            S.vs[j / AW_BLOCK] = vs;
-        }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        aw_math(p[h], g[h], m[h], v[h], root, s, k, keep);
+        aw_store<PE, FULL>(T.p, i + 1024 * h, T.n, p[h]);
+        aw_store<0, FULL>(mt, i + 1024 * h, T.n, m[h]);
+        aw_store<0, FULL>(vt, i + 1024 * h, T.n, v[h]);
     }
+}
+
+template <int BITS, int PE, int GE, bool FULL>
+__device__ __forceinline__ void aw_update(const AwTensor& T, const AwState& S, const void* g, long c0, const AwScal& s, float k, float keep)
+{
+    if constexpr (BITS == 8) {
+        const long i = c0 + threadIdx.x * 8;
+        if (FULL || i / AW_BLOCK * AW_BLOCK < T.n) aw_update8<PE, GE, FULL>(T, S, g, i, s, k, keep);
+    } else aw_update32<PE, GE, FULL>(T, S, g, c0 + threadIdx.x * 4, s, k, keep);
+}
+
+template <int BITS, int PE, int GE>
+__device__ __forceinline__ void aw_update(const AwTensor& T, const AwState& S, const void* g, int chunk, const AwScal& s, float k, float keep)
+{
+    const long c0 = (long)chunk * AW_CHUNK;
+    if (c0 + AW_CHUNK <= T.n) aw_update<BITS, PE, GE, true>(T, S, g, c0, s, k, keep);
+    else aw_update<BITS, PE, GE, false>(T, S, g, c0, s, k, keep);
 }
 
 template <int BITS>
@@ -192,26 +287,21 @@ __global__ __launch_bounds__(256) void k_adamw(const AwTensor* __restrict__ tens
         s.c2 = (float)scal[2];
     }
     const float keep = (float)(1.0 - s.lr * (double)T.decay);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int r = 0; r < AW_CHUNK / (4 * AW_BLOCK); r++) {
-        const long b0 = (long)ch.chunk * AW_CHUNK + (long)(r * 4 + wave) * AW_BLOCK;
-        if (b0 >= T.n) return;
-        const long i = b0 + lane * 4;
-        switch (T.ptype * 3 + T.gtype) {
-            case 0: aw_update<BITS, 0, 0>(T, S, g, i, lane, s, k, keep); break;
-            case 1: aw_update<BITS, 0, 1>(T, S, g, i, lane, s, k, keep); break;
-            case 2: aw_update<BITS, 0, 2>(T, S, g, i, lane, s, k, keep); break;
-            case 3: aw_update<BITS, 1, 0>(T, S, g, i, lane, s, k, keep); break;
-            case 4: aw_update<BITS, 1, 1>(T, S, g, i, lane, s, k, keep); break;
-            case 5: aw_update<BITS, 1, 2>(T, S, g, i, lane, s, k, keep); break;
-            case 6: aw_update<BITS, 2, 0>(T, S, g, i, lane, s, k, keep); break;
-            case 7: aw_update<BITS, 2, 1>(T, S, g, i, lane, s, k, keep); break;
-            default: aw_update<BITS, 2, 2>(T, S, g, i, lane, s, k, keep); break;
-        }
+    switch (T.ptype * 3 + T.gtype) {
+        case 0: aw_update<BITS, 0, 0>(T, S, g, ch.chunk, s, k, keep); break;
+        case 1: aw_update<BITS, 0, 1>(T, S, g, ch.chunk, s, k, keep); break;
+        case 2: aw_update<BITS, 0, 2>(T, S, g, ch.chunk, s, k, keep); break;
+        case 3: aw_update<BITS, 1, 0>(T, S, g, ch.chunk, s, k, keep); break;
+        case 4: aw_update<BITS, 1, 1>(T, S, g, ch.chunk, s, k, keep); break;
+        case 5: aw_update<BITS, 1, 2>(T, S, g, ch.chunk, s, k, keep); break;
+        case 6: aw_update<BITS, 2, 0>(T, S, g, ch.chunk, s, k, keep); break;
+        case 7: aw_update<BITS, 2, 1>(T, S, g, ch.chunk, s, k, keep); break;
+        default: aw_update<BITS, 2, 2>(T, S, g, ch.chunk, s, k, keep); break;
     }
 }
 
-// ---- the norm: float64 partial sums per workgroup, then one workgroup adds them in order ----
+// ---- the norm: float64 partial sums per workgroup, then one workgroup adds them in order (a launch of its own, 3 us: the last
+// workgroup of the first launch doing it costs every workgroup a release of its XCD's L2: 44 us for 1 M elements) ----
 __device__ __forceinline__ double aw_block_sum(double x, double* lds)
 {
     for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
@@ -222,6 +312,24 @@ __device__ __forceinline__ double aw_block_sum(double x, double* lds)
     return x;
 }
 
+template <int E, bool FULL> __device__ __forceinline__ double aw_square_sum(const void* g, long i, long n)
+{
+    float x[8];
+    aw_load<E, FULL>(g, i, n, x);
+    double a = 0.0, b = 0.0;
+#pragma unroll
+    for (int q = 0; q < 8; q += 2) {
+        a = fma((double)x[q], (double)x[q], a);
+        b = fma((double)x[q + 1], (double)x[q + 1], b);
+    }
+    return a + b;
+}
+template <bool FULL> __device__ __forceinline__ double aw_square_sum(int gtype, const void* g, long i, long n)
+{
+    return gtype == 0 ? aw_square_sum<0, FULL>(g, i, n) : gtype == 1 ? aw_square_sum<1, FULL>(g, i, n) : aw_square_sum<2, FULL>(g, i, n);
+}
+
+// add: a launch after the first of several
 __global__ __launch_bounds__(256) void k_adamw_sumsq(const AwTensor* __restrict__ tensors, const AwChunk* __restrict__ chunks, int n_chunks, int base,
                                                      AwGrads grads, double* __restrict__ partials, int add)
 {
@@ -231,15 +339,8 @@ __global__ __launch_bounds__(256) void k_adamw_sumsq(const AwTensor* __restrict_
         const AwChunk ch = chunks[b];
         const AwTensor& T = tensors[ch.tensor];
         const void* g = grads.g[ch.tensor - base];
-        if (!g) continue;
-        for (int r = 0; r < AW_CHUNK / 1024; r++) {
-            const long i = (long)ch.chunk * AW_CHUNK + r * 1024 + threadIdx.x * 4;
-            float x[4];
-            if (T.gtype == 0) aw_load<0>(g, i, T.n, x);
-            else if (T.gtype == 1) aw_load<1>(g, i, T.n, x);
-            else aw_load<2>(g, i, T.n, x);
-            for (int q = 0; q < 4; q++) sum = fma((double)x[q], (double)x[q], sum);
-        }
+        const long c0 = (long)ch.chunk * AW_CHUNK, i = c0 + threadIdx.x * 8, n = g ? T.n : 0;
+        sum += c0 + AW_CHUNK <= n ? aw_square_sum<true>(T.gtype, g, i, n) : aw_square_sum<false>(T.gtype, g, i, n);
     }
     sum = aw_block_sum(sum, lds);
     if (threadIdx.x == 0) partials[blockIdx.x] = add ? partials[blockIdx.x] + sum : sum;
@@ -255,7 +356,7 @@ __global__ __launch_bounds__(256) void k_adamw_norm(const double* __restrict__ p
     if (threadIdx.x == 0) {
         const double norm = sqrt(sum);
         out[0] = (float)norm;
-        out[1] = !(norm <= (double)INFINITY) || norm == (double)INFINITY ? NAN : norm > max_norm ? (float)(max_norm / norm) : 1.0f;
+        out[1] = !(norm < (double)INFINITY) ? NAN : norm > max_norm ? (float)(max_norm / norm) : 1.0f;
     }
 }
 
@@ -265,21 +366,17 @@ __global__ __launch_bounds__(256) void k_adamw_pack(const AwTensor* __restrict__
 {
     const AwChunk ch = chunks[blockIdx.x];
     const AwTensor T = tensors[ch.tensor];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int r = 0; r < AW_CHUNK / (4 * AW_BLOCK); r++) {
-        const long b0 = (long)ch.chunk * AW_CHUNK + (long)(r * 4 + wave) * AW_BLOCK;
-        if (b0 >= T.n) return;
-        const long i = b0 + lane * 4, j = T.start + i;
-        float m[4], v[4], ms, vs;
-        aw_load<0>(m_in + T.start, i, T.n, m);
-        aw_load<0>(v_in + T.start, i, T.n, v);
-        for (int q = 0; q < 4; q++) v[q] = sqrtf(v[q]);
-        ((unsigned*)S.m)[j / 4] = aw_pack_mean(m, ms);
-        ((unsigned*)S.v)[j / 4] = aw_pack_root(v, vs);
-        if (lane == 0) {
-            S.ms[j / AW_BLOCK] = ms;
-            S.vs[j / AW_BLOCK] = vs;
-        }
+    const long i = (long)ch.chunk * AW_CHUNK + threadIdx.x * 8, j = T.start + i;
+    if (i / AW_BLOCK * AW_BLOCK >= T.n) return;
+    float m[8], v[8], root[8], ms, vs;
+    aw_load<0>(m_in + T.start, i, T.n, m);
+    aw_load<0>(v_in + T.start, i, T.n, v);
+    aw_sqrt(v, root);
+    *(AwCodes*)((char*)S.m + j) = aw_pack_mean(m, ms);
+    *(AwCodes*)((char*)S.v + j) = aw_pack_root(root, vs);
+    if (j % AW_BLOCK == 0) {
+        S.ms[j / AW_BLOCK] = ms;
+        S.vs[j / AW_BLOCK] = vs;
     }
 }
 
@@ -287,11 +384,12 @@ __global__ __launch_bounds__(256) void k_adamw_pack(const AwTensor* __restrict__
 __global__ __launch_bounds__(256) void k_adamw_unpack(AwState S, float* __restrict__ m_out, float* __restrict__ v_out, long quads)
 {
     for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < quads; q += (long)gridDim.x * 256) {
-        float m[4], v[4];
-        aw_mean_of(((const unsigned*)S.m)[q], S.ms[q / (AW_BLOCK / 4)], m);
-        aw_root_of(((const unsigned*)S.v)[q], S.vs[q / (AW_BLOCK / 4)], v);
+        const float ms = S.ms[q / (AW_BLOCK / 4)], vs = S.vs[q / (AW_BLOCK / 4)];
+        float m[8], r[8];
+        aw_mean_of(AwCodes{ { ((const unsigned*)S.m)[q], 0 } }, ms, m);
+        aw_root_of(AwCodes{ { ((const unsigned*)S.v)[q], 0 } }, vs, r);
         ((float4*)m_out)[q] = make_float4(m[0], m[1], m[2], m[3]);
-        ((float4*)v_out)[q] = make_float4(v[0] * v[0], v[1] * v[1], v[2] * v[2], v[3] * v[3]);
+        ((float4*)v_out)[q] = make_float4(r[0] * r[0], r[1] * r[1], r[2] * r[2], r[3] * r[3]);
     }
 }
 
@@ -414,12 +512,10 @@ static int aw_check_grads(goai_ctx* c, const goai_adamw* o, const void* const* g
     return GOAI_OK;
 }
 
-int adamw_grad_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out)
+static int aw_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out)
 {
-    int rc = aw_check_grads(c, o, grads);
-    if (rc) return rc;
     const int grid = std::max(1, std::min(AW_NORM_BLOCKS, o->first.back()));
-    rc = aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
+    const int rc = aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
         k_adamw_sumsq<<<grid, 256, 0, c->stream>>>(o->d_tensors, chunks, n, base, g, o->d_partials, base != 0);
     });
     if (rc) return rc;
@@ -428,10 +524,16 @@ int adamw_grad_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double
     return GOAI_OK;
 }
 
-int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
-               const float* clip, const double* scalars)
+int adamw_grad_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out)
 {
     const int rc = aw_check_grads(c, o, grads);
+    return rc ? rc : aw_norm(c, o, grads, max_norm, out);
+}
+
+int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
+               double max_norm, float* clip, const double* scalars)
+{
+    int rc = aw_check_grads(c, o, grads);
     if (rc) return rc;
     if (!scalars) {
         hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
@@ -441,6 +543,7 @@ int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, 
             return GOAI_ERR_STATE;
         }
     }
+    if (max_norm > 0.0 && (rc = aw_norm(c, o, grads, max_norm, clip))) return rc;
     AwScal s{ lr, (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
               (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))), (float)(lr / (1.0 - pow(beta1, (double)t))) };
     return aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {

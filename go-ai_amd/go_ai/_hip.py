@@ -84,7 +84,7 @@ _SIGNATURES = {
                         ctypes.POINTER(c_void_p)],
     "goai_adamw_destroy": [c_void_p, c_void_p],
     "goai_adamw_grad_norm": [c_void_p, c_void_p, c_void_p, c_double, c_void_p],
-    "goai_adamw_step": [c_void_p, c_void_p, c_void_p, c_int64, c_double, c_double, c_double, c_double, c_void_p, c_void_p],
+    "goai_adamw_step": [c_void_p, c_void_p, c_void_p, c_int64, c_double, c_double, c_double, c_double, c_double, c_void_p, c_void_p],
     "goai_adamw_load_moments": [c_void_p, c_void_p, c_void_p, c_void_p],
     "goai_adamw_moments": [c_void_p, c_void_p, c_void_p, c_void_p],
     "goai_comm_unique_id": [c_void_p],

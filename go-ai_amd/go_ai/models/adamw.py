@@ -6,6 +6,9 @@ import torch
 
 BLOCK = 256          # elements that share one scale of an 8-bit moment
 
+_dtype_of, _shape_of = torch.Tensor.dtype.__get__, torch.Tensor.shape.__get__
+_device_of, _is_contiguous, _address_of = torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
 
 def _ctypes_table(ctype, values):
     return (ctype * max(len(values), 1))(*values)
@@ -93,7 +96,7 @@ class AdamW:
             scales[0].data_ptr() if eight else None, scales[1].data_ptr() if eight else None, ctypes.byref(h)))
         self._h = h
         self.params, self.device = params, device
-        self._gtypes, self._shapes = gtypes, [p.shape for p in params]
+        self._gtypes, self._shapes, self._devices = gtypes, [p.shape for p in params], [device.index] * n
         self._m, self._v, self._scales, self._elems = m, v, scales, elems
         self._table = _ctypes_table(ctypes.c_void_p, [None] * n)
         self._clip = torch.zeros(2, dtype=torch.float32, device=device)
@@ -126,15 +129,22 @@ class AdamW:
     def _grads(self, grads):
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW: {len(self.params)} parameters, {len(grads)} gradients")
-        table, device = self._table, self.device.index
+        try:                                                     # one pass per property: a third faster than tensor by tensor
+            if (list(map(_dtype_of, grads)) == self._gtypes and list(map(_shape_of, grads)) == self._shapes
+                    and list(map(_device_of, grads)) == self._devices and all(map(_is_contiguous, grads))):
+                self._table[:] = list(map(_address_of, grads))
+                return self._table
+        except TypeError:                                        # a gradient that is None
+            pass
+        table = self._table
         for i, (g, dtype, shape) in enumerate(zip(grads, self._gtypes, self._shapes)):
             if g is None:
                 table[i] = None
-            elif g.dtype is dtype and g.shape == shape and g.get_device() == device and g.is_contiguous():
+            elif torch.is_tensor(g) and g.dtype is dtype and g.shape == shape and g.device == self.device and g.is_contiguous():
                 table[i] = g.data_ptr()
             else:
-                raise ValueError(f"AdamW: gradient {i} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {self.device}, got {g.dtype} "
-                                 f"of shape {tuple(g.shape)} on {g.device}, strides {g.stride()}")
+                what = f"{g.dtype} of shape {tuple(g.shape)} on {g.device}, strides {g.stride()}" if torch.is_tensor(g) else type(g).__name__
+                raise ValueError(f"AdamW: gradient {i} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {self.device}, got {what}")
         return table
 
     def advance(self):
@@ -154,12 +164,9 @@ class AdamW:
         table = self._grads(grads)
         if captured and self._scalars is None:
             raise RuntimeError("AdamW: call advance() before a captured step")
-        clip = None
-        if self.max_norm:
-            clip = self._clip.data_ptr()
-            _hip.check(_hip.lib.goai_adamw_grad_norm(self._ctx._h, self._h, table, self.max_norm, clip))
         t = self.steps if captured else self.steps + 1
-        _hip.check(_hip.lib.goai_adamw_step(self._ctx._h, self._h, table, max(t, 1), self.lr, self.betas[0], self.betas[1], self.eps, clip,
+        _hip.check(_hip.lib.goai_adamw_step(self._ctx._h, self._h, table, max(t, 1), self.lr, self.betas[0], self.betas[1], self.eps,
+                                            self.max_norm, self._clip.data_ptr() if self.max_norm else None,
                                             self._scalars.data_ptr() if captured else None))
         self.steps = t
 
@@ -198,8 +205,7 @@ class AdamW:
         if self.state_bits == 8:
             flat = [torch.zeros(self._elems, dtype=torch.float32, device=self.device) for _ in range(2)]
         for to, given in zip(flat, (exp_avg, exp_avg_sq)):
-            for dst, src in zip(self._split(to), given):
-                dst.copy_(src)
+            torch._foreach_copy_(self._split(to), list(given))
         if self.state_bits == 8 and self._elems:
             from .. import _hip
             _hip.check(_hip.lib.goai_adamw_load_moments(self._ctx._h, self._h, flat[0].data_ptr(), flat[1].data_ptr()))

@@ -451,7 +451,8 @@ int goai_adamw_destroy(goai_ctx* ctx, goai_adamw* opt);
  * float64 in a fixed order.  max_norm = INFINITY: the norm alone. */
 int goai_adamw_grad_norm(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, double max_norm, float* norm_and_coef);
 
-/* Step number t (from 1): with g the gradient times the coefficient of norm_and_coef (DEVICE, may be NULL: 1),
+/* Step number t (from 1): with g the gradient times the coefficient of norm_and_coef (DEVICE float[2]; NULL: 1; max_norm > 0: the
+ * call computes it first, as goai_adamw_grad_norm does; max_norm = 0: it is as the caller left it),
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * in float32, rounded to the parameter's type and the moments' bits at the end.  A NaN coefficient leaves everything as it is,
@@ -461,7 +462,7 @@ int goai_adamw_grad_norm(goai_ctx* ctx, goai_adamw* opt, const void* const* grad
  * read when the step runs, in place of lr and t: a step that is captured into a graph needs it (GOAI_ERR_STATE without), and the
  * graph's owner updates it between replays.  Two calls on the same optimiser must not run at the same time. */
 int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, int64_t t, double lr, double beta1, double beta2,
-                    double eps, const float* norm_and_coef, const double* scalars);
+                    double eps, double max_norm, float* norm_and_coef, const double* scalars);
 
 /* Moments from / to float32 arrays [elems] of the flat layout (16-byte aligned), rounding to / reading the 8-bit codes. */
 int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* exp_avg, const float* exp_avg_sq);

@@ -96,10 +96,11 @@ def test_adamw_state_elems():
 
 def test_adamw_calls():
     table = (P * 1)(64)
-    step = lambda t=1, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, opt=64, g=table: lib.goai_adamw_step(None, opt, g, t, lr, b1, b2, eps, None, None)  # noqa: E731
+    step = lambda t=1, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, opt=64, g=table, m=0.0, c=None: lib.goai_adamw_step(None, opt, g, t, lr, b1, b2, eps, m, c, None)  # noqa: E731
     for bad, message in ((dict(t=0), "t = 1"), (dict(lr=-1.0), "lr"), (dict(lr=math.nan), "lr"), (dict(lr=math.inf), "lr"), (dict(b1=1.0), "betas"),
                          (dict(b2=-0.1), "betas"), (dict(b2=math.nan), "betas"), (dict(eps=0.0), "eps"), (dict(eps=math.nan), "eps"),
-                         (dict(opt=None), "NULL"), (dict(g=None), "NULL"), (dict(), "ctx is NULL")):
+                         (dict(opt=None), "NULL"), (dict(g=None), "NULL"), (dict(m=-1.0), "max_norm"), (dict(m=math.nan), "max_norm"),
+                         (dict(m=1.0), "norm_and_coef"), (dict(m=1.0, c=64), "ctx is NULL"), (dict(), "ctx is NULL")):
         assert step(**bad) == -1 and message in err(), bad
     norm = lambda m=1.0, opt=64, g=table, out=64: lib.goai_adamw_grad_norm(None, opt, g, m, out)  # noqa: E731
     for bad, message in ((dict(m=0.0), "max_norm"), (dict(m=-1.0), "max_norm"), (dict(m=math.nan), "max_norm"), (dict(opt=None), "NULL"),
