@@ -14,6 +14,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "ctx.h"
 #include "elem.h"
@@ -132,16 +133,34 @@ template <int L> __device__ __forceinline__ float lp_threshold(float lane_max, i
     return fmaxf(__shfl(s, (lane & (64 - L)) + top - 1), -FLT_MAX);
 }
 
-// bit (N - 1 - k) for x[k] >= t
+// bit (N - 1 - k) for x[k] >= t: bits = 2 bits + (x[k] >= t), a compare and an add with its carry.  The carry may be read two
+// instructions after the compare at the earliest, so compares and adds go four by four.
 template <int N> __device__ __forceinline__ unsigned lp_at_least(const float (&x)[N], float t)
 {
     unsigned bits = 0;
+    unsigned long long a, b, c, d, e;
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-        // bits = 2 bits + (x[k] >= t): a compare and an add with its carry
-        asm("v_cmp_ge_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(bits) : "v"(x[k]), "v"(t) : "vcc");
-    }
+    for (int k = 0; k + 4 <= N; k += 4)
+        asm("v_cmp_ge_f32 %1, %6, %10\n\tv_cmp_ge_f32 %2, %7, %10\n\tv_cmp_ge_f32 %3, %8, %10\n\tv_cmp_ge_f32 %4, %9, %10\n\t"
+            "v_addc_co_u32 %0, %5, %0, %0, %1\n\tv_addc_co_u32 %0, %5, %0, %0, %2\n\t"
+            "v_addc_co_u32 %0, %5, %0, %0, %3\n\tv_addc_co_u32 %0, %5, %0, %0, %4"
+            : "+v"(bits), "=&s"(a), "=&s"(b), "=&s"(c), "=&s"(d), "=&s"(e)
+            : "v"(x[k]), "v"(x[k + 1]), "v"(x[k + 2]), "v"(x[k + 3]), "v"(t));
+#pragma unroll
+    for (int k = N / 4 * 4; k < N; k++) bits = 2 * bits + (x[k] >= t ? 1u : 0u);
     return bits;
+}
+
+// x[k] = -inf where byte k of `ok` is 0 (as above: four compares, four selections)
+__device__ __forceinline__ void lp_mask4(float& x0, float& x1, float& x2, float& x3, unsigned ok)
+{
+    unsigned long long a, b, c, d;
+    asm("v_cmp_ne_u32_sdwa %4, %8, %9 src0_sel:BYTE_0 src1_sel:DWORD\n\tv_cmp_ne_u32_sdwa %5, %8, %9 src0_sel:BYTE_1 src1_sel:DWORD\n\t"
+        "v_cmp_ne_u32_sdwa %6, %8, %9 src0_sel:BYTE_2 src1_sel:DWORD\n\tv_cmp_ne_u32_sdwa %7, %8, %9 src0_sel:BYTE_3 src1_sel:DWORD\n\t"
+        "v_cndmask_b32 %0, %10, %0, %4\n\tv_cndmask_b32 %1, %10, %1, %5\n\tv_cndmask_b32 %2, %10, %2, %6\n\t"
+        "v_cndmask_b32 %3, %10, %3, %7"
+        : "+v"(x0), "+v"(x1), "+v"(x2), "+v"(x3), "=&s"(a), "=&s"(b), "=&s"(c), "=&s"(d)
+        : "v"(ok), "v"(0u), "v"(-INFINITY));
 }
 
 template <int L> __device__ __forceinline__ int lp_count(int n)
@@ -226,24 +245,19 @@ __device__ __forceinline__ bool lp_before(float v, int i, float w, int j) { retu
 constexpr int LP_NONE = 0x40000000;        // columns from here on stand for "no column" (with v = -inf): cols <= 2^30
 
 // How many of a group's L entries (one per lane, no two the same) come before the lane's own; L = 64: of the first `count`.
+template <int... K> __device__ __forceinline__ int lp_rank16(float v, int i, std::integer_sequence<int, K...>)
+{
+    // (rotations of the same register: no one waits for the one before)
+    return (0 + ... + (int)lp_before(lp_dpp<ROR + 1 + K>(v), lp_dpp<ROR + 1 + K>(i), v, i));
+}
 template <int L> __device__ __forceinline__ int lp_rank(float v, int i, int count)
 {
+    if constexpr (L == 16) return lp_rank16(v, i, std::make_integer_sequence<int, 15>());
     int rank = 0;
-    if constexpr (L == 16) {
-        float w = v;
-        int j = i;
-#pragma unroll
-        for (int k = 1; k < 16; k++) {
-            w = lp_dpp<ROR + 1>(w);
-            j = lp_dpp<ROR + 1>(j);
-            rank += lp_before(w, j, v, i);
-        }
-    } else {
-        for (int k = 0; k < count; k++) {
-            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k));
-            const int j = __builtin_amdgcn_readlane(i, k);
-            rank += lp_before(w, j, v, i);
-        }
+    for (int k = 0; k < count; k++) {
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k));
+        const int j = __builtin_amdgcn_readlane(i, k);
+        rank += lp_before(w, j, v, i);
     }
     return rank;
 }
@@ -343,23 +357,26 @@ template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_b
         ElemVec<E, V> t[NV];
 #pragma unroll
         for (int q = 0; q < NV; q++) __builtin_memcpy(&t[q], p + min((q * L + sub) * V, last), sizeof(t[q]));
+        unsigned ok[NV];                                         // a byte per column: not 0 where it is allowed
+#pragma unroll
+        for (int q = 0; q < NV; q++) ok[q] = ~0u;
         if (A.valid) {
             const uint8_t* valid = A.valid + row * A.vstride;
-            uint8_t ok[NV][V];
 #pragma unroll
-            for (int q = 0; q < NV; q++) __builtin_memcpy(ok[q], valid + min((q * L + sub) * V, last), V);
-#pragma unroll
-            for (int k = 0; k < N; k++) x[k] = ok[k / V][k % V] ? elem_to_float<E>(t[k / V].a[k % V]) : -INFINITY;
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; k++) x[k] = elem_to_float<E>(t[k / V].a[k % V]);
+            for (int q = 0; q < NV; q++) __builtin_memcpy(&ok[q], valid + min((q * L + sub) * V, last), V);
         }
 #pragma unroll
-        for (int q = 0; q < NV; q++) {
-            const int c = (q * L + sub) * V, cc = min(c, last);
-            if (q >= FULL) {
+        for (int k = 0; k < N; k++) x[k] = elem_to_float<E>(t[k / V].a[k % V]);
+        if (A.valid || FULL < NV) {
 #pragma unroll
-                for (int k = 0; k < V; k++) x[q * V + k] = cc + k >= c ? x[q * V + k] : -INFINITY;
+            for (int q = 0; q < NV; q++) {
+                if (!A.valid && q < FULL) continue;
+                if (q >= FULL) {
+                    const int c = (q * L + sub) * V;
+                    ok[q] &= (unsigned)(0xffffffffull << (8 * min(c - min(c, last), 4)));
+                }
+                if constexpr (V == 4) lp_mask4(x[q * V], x[q * V + 1], x[q * V + 2], x[q * V + 3], ok[q]);
+                else x[q] = ok[q] & 255u ? x[q] : -INFINITY;
             }
         }
     }
@@ -414,34 +431,6 @@ struct LpPart {                                            // a segment's result
     float m, l, e, pad;
 };
 
-// Sorted lists of `top` entries, list l at (lv, li) + l * top (one wavefront, lists <= 64): the best entries, best first, on the lanes
-__device__ __forceinline__ LpList lp_merge(const float* lv, const int* li, int lists, int top, int lane)
-{
-    LpList out;
-    int at = 0;
-    float v = lane < lists ? lv[lane * top] : -INFINITY;
-    int i = lane < lists ? li[lane * top] : LP_NONE + lane;
-    for (int r = 0; r < top; r++) {
-        float bv = v;
-        int bi = i;
-        for (int d = 1; d < lists; d <<= 1) {
-            const float w = __shfl_xor(bv, d);
-            const int j = __shfl_xor(bi, d);
-            if (lp_before(w, j, bv, bi)) { bv = w; bi = j; }
-        }
-        bv = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(bv)));
-        bi = __builtin_amdgcn_readfirstlane(bi);
-        if (bi >= LP_NONE) break;                          // nothing left
-        if (lane == r) { out.v = bv; out.i = bi; }
-        if (i == bi) {                                     // (columns differ: one lane)
-            at++;
-            v = at < top ? lv[lane * top + at] : -INFINITY;
-            i = at < top ? li[lane * top + at] : LP_NONE + lane;
-        }
-    }
-    return out;
-}
-
 // How many of a sorted list's `top` entries come before (v, i)
 __device__ __forceinline__ int lp_search(const float* lv, const int* li, int top, float v, int i)
 {
@@ -483,15 +472,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
             const int last = A.cols - V;
 #pragma unroll
             for (int q = 0; q < NV; q++) __builtin_memcpy(&u[q], p + min(base + (q * 64 + lane) * V, last), sizeof(u[q]));
+            unsigned ok[LP_E / 4];                         // a byte per column
             if (valid) {
-                uint8_t ok[NV][V];
 #pragma unroll
-                for (int q = 0; q < NV; q++) __builtin_memcpy(ok[q], valid + min(base + (q * 64 + lane) * V, last), V);
+                for (int q = 0; q < NV; q++) __builtin_memcpy(&ok[q * V / 4], valid + min(base + (q * 64 + lane) * V, last), V);
+            }
 #pragma unroll
-                for (int k = 0; k < LP_E; k++) x[k] = ok[k / V][k % V] ? elem_to_float<E>(u[k / V].a[k % V]) : -INFINITY;
-            } else {
+            for (int k = 0; k < LP_E; k++) x[k] = elem_to_float<E>(u[k / V].a[k % V]);
+            if (valid) {
 #pragma unroll
-                for (int k = 0; k < LP_E; k++) x[k] = elem_to_float<E>(u[k / V].a[k % V]);
+                for (int k = 0; k < LP_E; k += 4) lp_mask4(x[k], x[k + 1], x[k + 2], x[k + 3], ok[k / 4]);
             }
             if (base + LP_TILE > A.cols) {
 #pragma unroll
@@ -621,7 +611,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
 
 // The segments of a row together: one workgroup per row.  The lists come to LDS; of every list's entry number j (j as small as
 // `top` entries allow) the r-th largest is reached by `top` entries or more, few of them in general: they are the beginnings of their
-// lists, and are ranked as a short row's candidates are.  Where more than 64 are left, entry by entry (lp_merge).
+// lists, and are ranked as a short row's candidates are.
 template <int E, bool TOP>
 __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs A, int splits, const LpPart* __restrict__ parts, const float* __restrict__ part_v,
                                                        const int* __restrict__ part_i)
@@ -653,23 +643,37 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs A, int splits, con
         if (threadIdx.x >= 64) return;
         const int j = (top - 1) / splits, r = (top + j) / (j + 1);             // r lists with j + 1 entries each: r <= splits
         const float T = lp_threshold<64>(lane < splits ? lds_v[lane * top + j] : -INFINITY, r, lane);
-        int mine = lane < splits ? lp_search(lds_v + lane * top, lds_i + lane * top, top, T, LP_NONE) : 0;      // this list's entries >= T
-        const int at = lp_before_me<64>(mine, lane), count = __builtin_amdgcn_readlane(at + mine, 63);
-        if (count <= 64) {
-            for (int k = 0; k < mine; k++) {
-                cand_v[at + k] = lds_v[lane * top + k];
-                cand_i[at + k] = lds_i[lane * top + k];
-            }
-            lp_wave_sync();
-            const float v = lane < count ? cand_v[lane] : -INFINITY;
-            const int i = lane < count ? cand_i[lane] : LP_NONE + lane;
-            int rank = lp_rank<64>(v, i, count);
-            if (lane >= count) rank = lane;
-            if (rank < top) lp_write_top(A, row, rank, v, i, s, logl);
-        } else {
-            const LpList t = lp_merge(lds_v, lds_i, splits, top, lane);
-            if (lane < top) lp_write_top(A, row, lane, t.v, t.i, s, logl);
+        // entries of this lane's list that come before (t, i)
+        const auto reach = [&](float t, int i) { return lane < splits ? lp_search(lds_v + lane * top, lds_i + lane * top, top, t, i) : 0; };
+        int mine = reach(T, LP_NONE), count = __builtin_amdgcn_readfirstlane(lp_count<64>(mine));      // those that are >= T
+        if (count > 64) {                                  // halved as in lp_candidates: values, then columns of one value
+            const auto halve = [&](int lo, int hi, auto&& before) {
+                while (count > 64 && (unsigned)hi - (unsigned)lo > 1u) {
+                    const int mid = __builtin_amdgcn_readfirstlane((int)((unsigned)lo + (((unsigned)hi - (unsigned)lo) >> 1)));
+                    const int m = before(mid), n = __builtin_amdgcn_readfirstlane(lp_count<64>(m));
+                    if (n >= top) {
+                        lo = mid;
+                        mine = m;
+                        count = n;
+                    } else hi = mid;
+                }
+                return lo;
+            };
+            const int lo = halve(lp_key(__float_as_int(T)), lp_key(__float_as_int(s.m)) + 1,
+                                 [&](int mid) { return reach(__int_as_float(lp_key(mid)), LP_NONE); });
+            halve(-LP_NONE, 0, [&](int mid) { return reach(__int_as_float(lp_key(lo)), -mid); });      // (the fewer, the larger mid)
         }
+        const int at = lp_before_me<64>(mine, lane);
+        for (int k = 0; k < mine; k++) {
+            cand_v[at + k] = lds_v[lane * top + k];
+            cand_i[at + k] = lds_i[lane * top + k];
+        }
+        lp_wave_sync();
+        const float v = lane < count ? cand_v[lane] : -INFINITY;
+        const int i = lane < count ? cand_i[lane] : LP_NONE + lane;
+        int rank = lp_rank<64>(v, i, count);
+        if (lane >= count) rank = lane;
+        if (rank < top) lp_write_top(A, row, rank, v, i, s, logl);
     }
 }
 
@@ -877,7 +881,7 @@ template <int E, int L, int V> static void lp_launch_grad(LpGradArgs A, hipStrea
 template <int E> static void lp_launch_grad(const LpGradArgs& A, hipStream_t st)
 {
     constexpr int V = E == 0 ? 4 : 8;                   // 16 bytes; 8 of a short row, which has few vectors for its lanes (300000 x 26
-    if (A.cols < 4) lp_launch_grad<E, 16, 1>(A, st);    // bfloat16: TIMEC us, with 16 bytes 30)
+    if (A.cols < 4) lp_launch_grad<E, 16, 1>(A, st);    // bfloat16: 21 us, with 16 bytes 30)
     else if (A.cols <= LG_N * 16 * 4) lp_launch_grad<E, 16, 4>(A, st);
     else if (A.cols <= LG_N * 16 * V) lp_launch_grad<E, 16, V>(A, st);
     else if (A.cols <= LG_N * 64 * V) lp_launch_grad<E, 64, V>(A, st);
