@@ -411,7 +411,42 @@ int goai_train_step(goai_ctx* ctx, const uint8_t* states, const uint8_t* next_st
                     int n, float lr, float weight_decay, float* metrics_host)
 {
     CTX_ENTER(ctx);
-    return train_step(ctx, states, next_states, wins, pi, n, lr, weight_decay, metrics_host);
+    return train_step(ctx, states, next_states, wins, pi, n, lr, weight_decay, metrics_host, true);
+}
+
+int goai_train_backward(goai_ctx* ctx, const uint8_t* states, const uint8_t* next_states, const float* wins, const float* pi, int n,
+                        float* metrics_host)
+{
+    CTX_ENTER(ctx);
+    return train_step(ctx, states, next_states, wins, pi, n, 0.0f, 0.0f, metrics_host, false);
+}
+
+int goai_train_actor_forward(goai_ctx* ctx, const uint8_t* states, float* logits, int n)
+{
+    CTX_ENTER(ctx);
+    return train_actor_forward(ctx, states, logits, n);
+}
+
+int goai_train_actor_backward(goai_ctx* ctx, const float* d_logits, int n)
+{
+    CTX_ENTER(ctx);
+    return train_actor_backward(ctx, d_logits, n);
+}
+
+int goai_train_parameter(goai_ctx* ctx, const char* name, int64_t* offset, int64_t* numel)
+{
+    CTX_ENTER(ctx);
+    return train_parameter(ctx, name, offset, numel);
+}
+
+int goai_train_grads(goai_ctx* ctx, float** grads_device, int64_t* numel)
+{
+    CTX_ENTER(ctx);
+    GOAI_REQUIRE(ctx->train.ready, "call goai_train_init first");
+    GOAI_REQUIRE(grads_device && numel, "NULL output");
+    *grads_device = ctx->train.grads;
+    *numel = (int64_t)ctx->train.n_params;
+    return GOAI_OK;
 }
 
 int goai_train_params(goai_ctx* ctx, float** params_device, int64_t* numel)
@@ -566,7 +601,6 @@ int goai_adamw_init(goai_ctx* ctx, int n_tensors, void* const* params, const int
 int goai_adamw_destroy(goai_ctx* ctx, goai_adamw* opt)
 {
     if (!opt) return GOAI_OK;
-    CTX_ENTER(ctx);
     return adamw_destroy(ctx, opt);
 }
 

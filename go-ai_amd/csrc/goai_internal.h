@@ -63,7 +63,10 @@ int train_load(goai_ctx* c, const char* const* names, const float* const* tensor
 int train_reset_optimizer(goai_ctx* c);
 int train_export(goai_ctx* c, int what, const char* const* names, float* const* tensors, const int64_t* numels, int n);
 int train_step(goai_ctx* c, const uint8_t* states, const uint8_t* next_states, const float* wins, const float* pi, int n, float lr,
-               float weight_decay, float* metrics_host);
+               float weight_decay, float* metrics_host, bool update);
+int train_actor_forward(goai_ctx* c, const uint8_t* states, float* logits, int n);
+int train_actor_backward(goai_ctx* c, const float* d_logits, int n);
+int train_parameter(goai_ctx* c, const char* name, int64_t* offset, int64_t* numel);
 int train_sync_inference(goai_ctx* c);
 
 // ---- result gather over ranks (gather.hip) ----

@@ -45,7 +45,8 @@ struct Train {
     float *in_wins = nullptr, *in_pi = nullptr;         // [max_batch], [max_batch][A]
     float* scal = nullptr;                              // device: lr, weight decay, 1 - 0.9^t, sqrt(1 - 0.999^t)
     float scal_host[4] = { 0.0f, 0.0f, 1.0f, 1.0f };
-    std::map<int, hipGraphExec_t> graphs;               // by batch size
+    std::map<int, hipGraphExec_t> graphs;               // by batch size; its negative: the step without the optimiser
+    int actor_rows = 0;                                 // positions of the actor pass that waits for its backward half, 0: none
     hipStream_t gstream = nullptr;                      // the step's own stream when the context runs on the null stream (which cannot be captured)
 };
 

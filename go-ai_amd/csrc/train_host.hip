@@ -327,32 +327,55 @@ int critic_pass(const Pass& p, const uint8_t* states, const float* wins, float w
     return trunk_backward(p, states);
 }
 
-// actor_step (models/__init__.py:167-186) through act_head
-int actor_pass(const Pass& p, const uint8_t* states, const float* pi)
+// the actor's logits of `states` (act_head), left in t.logits
+int actor_forward(const Pass& p, const uint8_t* states)
 {
     Train& t = p.t;
     const std::string h = "act_head";
     const int hb = 2 * t.layers + 1;
-    float* xl = t.x[t.layers];
     TR_TRY(trunk_forward(p, states));
-    TR_TRY(tr_head_fwd(xl, p.par(h + ".0.weight"), p.par(h + ".0.bias"), p.par(h + ".1.weight"), p.par(h + ".1.bias"), t.hz,
+    TR_TRY(tr_head_fwd(t.x[t.layers], p.par(h + ".0.weight"), p.par(h + ".0.bias"), p.par(h + ".1.weight"), p.par(h + ".1.bias"), t.hz,
                        p.mean(hb), p.invstd(hb), p.stat(h + ".1.running_mean"), p.stat(h + ".1.running_var"), t.f, p.M, 2, p.P, p.st));
-    TR_TRY(tr_linear_fwd(t.f, p.par(h + ".4.weight"), p.par(h + ".4.bias"), t.logits, p.n, p.A, 2 * p.P, 0, p.st));
-    TR_TRY(tr_actor_loss(t.logits, pi, t.dlogits, t.metrics, p.n, p.A, p.st));
+    return tr_linear_fwd(t.f, p.par(h + ".4.weight"), p.par(h + ".4.bias"), t.logits, p.n, p.A, 2 * p.P, 0, p.st);
+}
+
+// from the logits' gradient in t.dlogits
+int actor_backward(const Pass& p, const uint8_t* states)
+{
+    Train& t = p.t;
+    const std::string h = "act_head";
+    const int hb = 2 * t.layers + 1;
     TR_TRY(tr_linear_bwd(t.dlogits, t.f, p.par(h + ".4.weight"), nullptr, p.grad(h + ".4.weight"), p.grad(h + ".4.bias"), t.df, p.n,
                          p.A, 2 * p.P, p.st));
-    TR_TRY(tr_head_bwd(t.df, t.f, t.hz, p.mean(hb), p.invstd(hb), p.par(h + ".1.weight"), xl, p.par(h + ".0.weight"), t.col_partial,
-                       p.grad(h + ".1.weight"), p.grad(h + ".1.bias"), p.grad(h + ".0.weight"), p.grad(h + ".0.bias"), t.dhz, t.g[0],
-                       p.M, 2, p.P, p.st));
+    TR_TRY(tr_head_bwd(t.df, t.f, t.hz, p.mean(hb), p.invstd(hb), p.par(h + ".1.weight"), t.x[t.layers], p.par(h + ".0.weight"),
+                       t.col_partial, p.grad(h + ".1.weight"), p.grad(h + ".1.bias"), p.grad(h + ".0.weight"), p.grad(h + ".0.bias"), t.dhz,
+                       t.g[0], p.M, 2, p.P, p.st));
     return trunk_backward(p, states);
+}
+
+// actor_step (models/__init__.py:167-186) through act_head
+int actor_pass(const Pass& p, const uint8_t* states, const float* pi)
+{
+    TR_TRY(actor_forward(p, states));
+    TR_TRY(tr_actor_loss(p.t.logits, pi, p.t.dlogits, p.t.metrics, p.n, p.A, p.st));
+    return actor_backward(p, states);
+}
+
+// the convolutions' weights as the kernels read them
+int relayout(const Pass& p)
+{
+    const size_t img = (size_t)9 * 128 * 128;
+    for (int l = 1; l <= 2 * p.t.layers; l++)
+        TR_TRY(tr_relayout(p.par(trunk_names(l).conv + ".weight"), p.t.img_f + (size_t)(l - 1) * img, p.t.img_d + (size_t)(l - 1) * img, p.st));
+    return GOAI_OK;
 }
 }  // namespace
 
-// One train_step.  states / next_states: device uint8 [n][6][S][S]; wins: device float [n]; pi: device float [n][A]
-// (actor-critic only; states and pi are ignored for the value net).  metrics_host: critic loss, critic accuracy,
+// One train_step, or (update = false) its gradients alone.  states / next_states: device uint8 [n][6][S][S]; wins: device
+// float [n]; pi: device float [n][A] (actor-critic only; states and pi are ignored for the value net).  metrics_host: critic loss, critic accuracy,
 // actor loss, actor accuracy (NaN for the value net's actor entries).
 int train_step(goai_ctx* c, const uint8_t* states, const uint8_t* next_states, const float* wins, const float* pi, int n, float lr,
-               float weight_decay, float* metrics_host)
+               float weight_decay, float* metrics_host, bool update)
 {
     Train& t = c->train;
     GOAI_REQUIRE(t.ready, "call goai_train_init first");
@@ -367,7 +390,9 @@ int train_step(goai_ctx* c, const uint8_t* states, const uint8_t* next_states, c
         st = t.gstream;
     }
     const Pass p{ c, t, c->S, c->P, c->A, n, n * c->P, st };
-    t.steps++;
+    const int key = update ? n : -n;
+    t.actor_rows = 0;
+    if (update) t.steps++;
     const double bc1 = 1.0 - std::pow(0.9, (double)t.steps), bc2 = 1.0 - std::pow(0.999, (double)t.steps);
     t.scal_host[0] = lr;
     t.scal_host[1] = weight_decay;
@@ -376,13 +401,12 @@ int train_step(goai_ctx* c, const uint8_t* states, const uint8_t* next_states, c
     GOAI_HIP_CHECK(hipMemcpyAsync(t.scal, t.scal_host, sizeof(t.scal_host), hipMemcpyHostToDevice, p.st));
     // everything between the caller's arrays and the metrics: the same launches for every step of one batch size
     auto body = [&](const uint8_t* st_in, const uint8_t* nx_in, const float* wins_in, const float* pi_in) -> int {
-        const size_t img = (size_t)9 * 128 * 128;
         TR_TRY(tr_fill(t.grads, (long)t.n_params, 0.0f, p.st));                                  // optimizer.zero_grad()
         TR_TRY(tr_fill(t.metrics, 4, NAN, p.st));
-        for (int l = 1; l <= 2 * t.layers; l++)
-            TR_TRY(tr_relayout(p.par(trunk_names(l).conv + ".weight"), t.img_f + (size_t)(l - 1) * img, t.img_d + (size_t)(l - 1) * img, p.st));
+        TR_TRY(relayout(p));
         TR_TRY(critic_pass(p, nx_in, wins_in, t.kind == 0 ? 2.0f : 1.0f));
         if (t.kind == 0) TR_TRY(actor_pass(p, st_in, pi_in));
+        if (!update) return GOAI_OK;
         return tr_adam(t.params, t.grads, t.adam_m, t.adam_v, (long)t.n_params, t.scal, p.st);
     };
     int rc = GOAI_OK;
@@ -394,7 +418,7 @@ int train_step(goai_ctx* c, const uint8_t* states, const uint8_t* next_states, c
         }
         GOAI_HIP_CHECK(hipMemcpyAsync(t.in_next, next_states, sb, hipMemcpyDeviceToDevice, p.st));
         GOAI_HIP_CHECK(hipMemcpyAsync(t.in_wins, wins, (size_t)n * sizeof(float), hipMemcpyDeviceToDevice, p.st));
-        auto it = t.graphs.find(n);
+        auto it = t.graphs.find(key);
         if (it == t.graphs.end()) {
             // first step of this batch size: record the launches (nothing runs while the stream is capturing)
             hipGraph_t graph = nullptr;
@@ -414,18 +438,68 @@ int train_step(goai_ctx* c, const uint8_t* states, const uint8_t* next_states, c
                 }
             }
             if (graph) (void)hipGraphDestroy(graph);
-            if (rc == GOAI_OK) it = t.graphs.emplace(n, exec).first;
+            if (rc == GOAI_OK) it = t.graphs.emplace(key, exec).first;
         }
         if (rc == GOAI_OK) GOAI_HIP_CHECK(hipGraphLaunch(it->second, p.st));
     } else
         rc = body(states, next_states, wins, pi);
     if (rc != GOAI_OK) {
-        t.steps--;
+        if (update) t.steps--;
         (void)hipStreamSynchronize(p.st);
         return rc;
     }
     GOAI_HIP_CHECK(hipMemcpyAsync(metrics_host, t.metrics, 4 * sizeof(float), hipMemcpyDeviceToHost, p.st));
     GOAI_HIP_CHECK(hipStreamSynchronize(p.st));
+    return GOAI_OK;
+}
+
+// The actor's logits of n positions in training mode; the activations wait for train_actor_backward.
+int train_actor_forward(goai_ctx* c, const uint8_t* states, float* logits, int n)
+{
+    Train& t = c->train;
+    GOAI_REQUIRE(t.ready, "call goai_train_init first");
+    GOAI_REQUIRE(t.kind == 0, "the value net has no policy head");
+    GOAI_REQUIRE(n >= 2 && n <= t.max_batch, "batch size must be in 2 .. max_batch");
+    GOAI_REQUIRE(states && logits, "NULL array argument");
+    const Pass p{ c, t, c->S, c->P, c->A, n, n * c->P, c->stream };
+    t.actor_rows = 0;
+    GOAI_HIP_CHECK(hipMemcpyAsync(t.in_states, states, (size_t)n * 6 * c->P, hipMemcpyDeviceToDevice, p.st));
+    TR_TRY(relayout(p));
+    TR_TRY(actor_forward(p, t.in_states));
+    GOAI_HIP_CHECK(hipMemcpyAsync(logits, t.logits, (size_t)n * c->A * sizeof(float), hipMemcpyDeviceToDevice, p.st));
+    t.actor_rows = n;
+    return GOAI_OK;
+}
+
+int train_actor_backward(goai_ctx* c, const float* d_logits, int n)
+{
+    Train& t = c->train;
+    GOAI_REQUIRE(t.ready, "call goai_train_init first");
+    GOAI_REQUIRE(d_logits != nullptr, "NULL array argument");
+    if (t.actor_rows != n || n == 0) {
+        set_error("goai_train_actor_backward must follow goai_train_actor_forward of the same positions");
+        return GOAI_ERR_STATE;
+    }
+    const Pass p{ c, t, c->S, c->P, c->A, n, n * c->P, c->stream };
+    t.actor_rows = 0;
+    TR_TRY(tr_fill(t.grads, (long)t.n_params, 0.0f, p.st));
+    GOAI_HIP_CHECK(hipMemcpyAsync(t.dlogits, d_logits, (size_t)n * c->A * sizeof(float), hipMemcpyDeviceToDevice, p.st));
+    return actor_backward(p, t.in_states);
+}
+
+// place of a named parameter in the flat parameter and gradient buffers
+int train_parameter(goai_ctx* c, const char* name, int64_t* offset, int64_t* numel)
+{
+    Train& t = c->train;
+    GOAI_REQUIRE(t.ready, "call goai_train_init first");
+    GOAI_REQUIRE(name && offset && numel, "NULL argument");
+    auto it = t.slots.find(name);
+    if (it == t.slots.end() || it->second.stat) {
+        set_error(std::string("the training net has no parameter ") + name);
+        return GOAI_ERR_ARG;
+    }
+    *offset = (int64_t)it->second.off;
+    *numel = (int64_t)it->second.numel;
     return GOAI_OK;
 }
 

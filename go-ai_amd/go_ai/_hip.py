@@ -72,6 +72,11 @@ _SIGNATURES = {
     "goai_train_reset_optimizer": [c_void_p],
     "goai_train_step": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, ctypes.c_float, ctypes.c_float,
                         ctypes.POINTER(ctypes.c_float)],
+    "goai_train_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, ctypes.POINTER(ctypes.c_float)],
+    "goai_train_actor_forward": [c_void_p, c_void_p, c_void_p, c_int],
+    "goai_train_actor_backward": [c_void_p, c_void_p, c_int],
+    "goai_train_parameter": [c_void_p, ctypes.c_char_p, ctypes.POINTER(c_int64), ctypes.POINTER(c_int64)],
+    "goai_train_grads": [c_void_p, ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64)],
     "goai_train_params": [c_void_p, ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64)],
     "goai_train_sync_inference": [c_void_p],
     "goai_action_logprobs": [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_double, c_int, c_void_p, c_void_p, c_void_p,

@@ -340,9 +340,7 @@ class Context:
         self._bind()
         _hip.check(_hip.lib.goai_train_reset_optimizer(self._h))
 
-    def train_step(self, states, next_states, wins, pi, lr=1e-3, weight_decay=1e-4):
-        """goai_train_step; returns (critic_loss, critic_acc, actor_loss, actor_acc), the last two None for the value net."""
-        self._bind()
+    def _train_batch(self, states, next_states, wins, pi):
         nxt = _dev_u8_states(next_states, self.device)
         n = nxt.shape[0]
         w = torch.as_tensor(np.asarray(wins, dtype=np.float32) if not torch.is_tensor(wins) else wins)
@@ -354,11 +352,61 @@ class Context:
             p = p.to(self.device, dtype=torch.float32).contiguous()
             assert st.shape[0] == n and tuple(p.shape) == (n, self.A), (st.shape, p.shape)
         assert w.numel() == n
+        return st, nxt, w, p, n
+
+    @staticmethod
+    def _train_metrics(m):
+        vals = [float(x) for x in m]
+        return tuple(None if np.isnan(v) else v for v in vals)
+
+    def train_step(self, states, next_states, wins, pi, lr=1e-3, weight_decay=1e-4):
+        """goai_train_step; returns (critic_loss, critic_acc, actor_loss, actor_acc), the last two None for the value net."""
+        self._bind()
+        st, nxt, w, p, n = self._train_batch(states, next_states, wins, pi)
         m = (ctypes.c_float * 4)()
         _hip.check(_hip.lib.goai_train_step(self._h, _hip.ptr(st), _hip.ptr(nxt), _hip.ptr(w), _hip.ptr(p), n,
                                             float(lr), float(weight_decay), m))
-        vals = [float(x) for x in m]
-        return tuple(None if np.isnan(v) else v for v in vals)
+        return self._train_metrics(m)
+
+    def train_backward(self, states, next_states, wins, pi):
+        """goai_train_backward: train_step's losses and gradients (train_grads) without the optimiser."""
+        self._bind()
+        st, nxt, w, p, n = self._train_batch(states, next_states, wins, pi)
+        m = (ctypes.c_float * 4)()
+        _hip.check(_hip.lib.goai_train_backward(self._h, _hip.ptr(st), _hip.ptr(nxt), _hip.ptr(w), _hip.ptr(p), n, m))
+        return self._train_metrics(m)
+
+    def train_actor_forward(self, states):
+        """goai_train_actor_forward: the actor's logits [n, A] in training mode."""
+        self._bind()
+        st = _dev_u8_states(states, self.device)
+        logits = torch.empty((st.shape[0], self.A), dtype=torch.float32, device=self.device)
+        _hip.check(_hip.lib.goai_train_actor_forward(self._h, _hip.ptr(st), _hip.ptr(logits), st.shape[0]))
+        return logits
+
+    def train_actor_backward(self, d_logits):
+        """goai_train_actor_backward: the parameters' gradients (train_grads) from train_actor_forward's logits' gradient."""
+        self._bind()
+        assert d_logits.dim() == 2 and d_logits.shape[1] == self.A and d_logits.dtype == torch.float32
+        _hip.check(_hip.lib.goai_train_actor_backward(self._h, _hip.ptr(d_logits), d_logits.shape[0]))
+
+    def train_parameter(self, name):
+        """(offset, numel) of a parameter in train_params() and train_grads()."""
+        off, n = ctypes.c_int64(), ctypes.c_int64()
+        _hip.check(_hip.lib.goai_train_parameter(self._h, name.encode(), ctypes.byref(off), ctypes.byref(n)))
+        return off.value, n.value
+
+    def _device_view(self, pointer, numel):
+        class _View:
+            __cuda_array_interface__ = {"shape": (numel,), "typestr": "<f4", "data": (pointer, False), "version": 2}
+        return torch.as_tensor(_View(), device=self.device)
+
+    def train_grads(self):
+        """The flat fp32 gradient buffer as a torch DEVICE tensor (a view, not a copy)."""
+        self._bind()
+        p, n = ctypes.c_void_p(), ctypes.c_int64()
+        _hip.check(_hip.lib.goai_train_grads(self._h, ctypes.byref(p), ctypes.byref(n)))
+        return self._device_view(p.value, n.value)
 
     def train_params(self):
         """The flat fp32 parameter buffer as a torch DEVICE tensor (a view, not a copy): all-reduce it in place to
@@ -366,10 +414,7 @@ class Context:
         self._bind()
         p, n = ctypes.c_void_p(), ctypes.c_int64()
         _hip.check(_hip.lib.goai_train_params(self._h, ctypes.byref(p), ctypes.byref(n)))
-
-        class _View:
-            __cuda_array_interface__ = {"shape": (n.value,), "typestr": "<f4", "data": (p.value, False), "version": 2}
-        return torch.as_tensor(_View(), device=self.device)
+        return self._device_view(p.value, n.value)
 
     def train_sync_inference(self):
         self._bind()

@@ -209,6 +209,26 @@ class RLNet:
         self._train_dirty = True
         return self._train.train_params()
 
+    def _bind_optimizer(self, optimizer):
+        """An AdamW without parameters of its own (or of this net's training state before it was rebuilt) takes this net's."""
+        if optimizer.params is not None and optimizer._ctx is self._train:
+            return
+        if optimizer.params is not None and getattr(optimizer, "_net", None) is not self:
+            raise ValueError("this AdamW already belongs to other parameters: a net needs one of its own (AdamW(None, ...))")
+        if optimizer.params is not None:
+            import warnings
+            warnings.warn("go_ai.models: the training state was rebuilt: AdamW's moments were reset", RuntimeWarning)
+        flat, grads = self._train.train_params(), self._train.train_grads()
+        params, optimizer._net_grads, optimizer._net_names = [], [], []
+        for k, shape in self._tensor_shapes().items():
+            if not k.endswith(("running_mean", "running_var")):
+                off, n = self._train.train_parameter(k)
+                params.append(flat[off:off + n].view(shape))
+                optimizer._net_grads.append(grads[off:off + n].view(shape))
+                optimizer._net_names.append(k)
+        optimizer.bind(params, self._train)
+        optimizer._net = self
+
     def train_step(self, optimizer, states, actions, reward, children, terminal, wins, pi):
         """One optimisation step on a batch of events (ac_net.py:67-86 / val_net.py:29-43): the critic learns -wins on
         next_states = children[actions] under random board symmetries, the actor (actor-critic net) argmax(pi) on
@@ -226,6 +246,12 @@ class RLNet:
         next_states = data.batch_random_symmetries(next_states)          # train_step's own
         next_states = data.batch_random_symmetries(next_states)          # critic_step's (models/__init__.py:119)
         self._train_dirty = True
+        if isinstance(optimizer, AdamW):
+            self._bind_optimizer(optimizer)
+            metrics = self._train.train_backward(states if self.kind == "ac" else None, next_states, np.asarray(wins, dtype=np.float32),
+                                                 pi if self.kind == "ac" else None)
+            optimizer.step(optimizer._net_grads)
+            return metrics
         return self._train.train_step(states if self.kind == "ac" else None, next_states, np.asarray(wins, dtype=np.float32),
                                       pi if self.kind == "ac" else None, lr=optimizer.lr, weight_decay=optimizer.weight_decay)
 

@@ -109,9 +109,9 @@ class AdamW:
         return self
 
     def close(self):
-        if self._h is not None and self._ctx is not None and not self._ctx.closed:
+        if self._h is not None:
             from .. import _hip
-            _hip.lib.goai_adamw_destroy(self._ctx._h, self._h)
+            _hip.lib.goai_adamw_destroy(None if self._ctx.closed else self._ctx._h, self._h)
         self._h = None
 
     def __del__(self):

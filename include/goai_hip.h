@@ -374,6 +374,23 @@ int goai_train_reset_optimizer(goai_ctx* ctx);
 int goai_train_step(goai_ctx* ctx, const uint8_t* states, const uint8_t* next_states, const float* wins,
                     const float* pi, int n, float lr, float weight_decay, float* metrics_host);
 
+/* goai_train_step without the optimiser: the step's losses and accuracies, its gradients in the flat buffer of goai_train_grads and
+ * its moves of the BatchNorm statistics; parameters, Adam's moments and step count stay. */
+int goai_train_backward(goai_ctx* ctx, const uint8_t* states, const uint8_t* next_states, const float* wins, const float* pi, int n,
+                        float* metrics_host);
+
+/* The actor alone, for losses of the caller's own (actor-critic net): its logits [n][A] of n positions in training mode (BatchNorm on
+ * the batch's statistics, the running ones move), and from the loss's gradient with respect to them all parameters' gradients
+ * (0 for the critic's head) in the flat buffer of goai_train_grads.  The backward call follows its forward call on the
+ * same context with no training call in between (else GOAI_ERR_STATE).  2 <= n <= max_batch.  Asynchronous. */
+int goai_train_actor_forward(goai_ctx* ctx, const uint8_t* states, float* logits, int n);
+int goai_train_actor_backward(goai_ctx* ctx, const float* d_logits, int n);
+
+/* Where the parameter `name` (a state_dict key; not a BatchNorm statistic) lies in the flat buffers of goai_train_params and
+ * goai_train_grads, in floats.  The gradients' buffer holds what the last step or backward call left. */
+int goai_train_parameter(goai_ctx* ctx, const char* name, int64_t* offset, int64_t* numel);
+int goai_train_grads(goai_ctx* ctx, float** grads_device, int64_t* numel);
+
 /* The flat fp32 DEVICE buffer of all parameters (not the BatchNorm statistics), for
  * average_model (/root/reference/go_ai/models/__init__.py:279-282): all-reduce it in place
  * over the ranks (RCCL) and scale by 1 / world_size.  Same layout on every rank. */
@@ -443,7 +460,7 @@ int64_t goai_adamw_state_elems(int n_tensors, const int64_t* numels);
 int goai_adamw_init(goai_ctx* ctx, int n_tensors, void* const* params, const int32_t* param_types, const int32_t* grad_types,
                     const int64_t* numels, const float* weight_decays, int state_bits, void* exp_avg, void* exp_avg_sq,
                     float* avg_scales, float* sq_scales, goai_adamw** out);
-/* Synchronises the stream. */
+/* Synchronises the stream; ctx may be NULL once its context is gone (then the GPU). */
 int goai_adamw_destroy(goai_ctx* ctx, goai_adamw* opt);
 
 /* The 2-norm over all gradients (grads: HOST table of DEVICE pointers; NULL: the tensor has none) and the clipping coefficient
