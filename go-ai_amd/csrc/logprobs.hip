@@ -51,35 +51,59 @@ __device__ __forceinline__ void lp_raise(LpStat& s, float m, LpFactor c)     // 
     s.m = m;
 }
 
-// ---- cross-lane helpers: lanes in rows of 16 by DPP, beyond that by shuffles ----
+// ---- cross-lane helpers: DPP moves within rows of 16 lanes and from row to row (no LDS unit: some 8 cycles a step against
+// some 100 of a shuffle) ----
 template <int CTRL> __device__ __forceinline__ int lp_dpp(int x) { return __builtin_amdgcn_mov_dpp(x, CTRL, 0xf, 0xf, true); }
 template <int CTRL> __device__ __forceinline__ float lp_dpp(float x) { return __int_as_float(lp_dpp<CTRL>(__float_as_int(x))); }
-constexpr int ROR = 0x120, MIRROR = 0x140, HALF_MIRROR = 0x141, XOR1 = 0xb1, XOR2 = 0x4e, XOR3 = 0x1b;
+constexpr int SHR = 0x110, ROR = 0x120, WAVE_SHR1 = 0x138, MIRROR = 0x140, HALF_MIRROR = 0x141, XOR1 = 0xb1, XOR2 = 0x4e, XOR3 = 0x1b;
+// lane 15 of each row to the row behind it (rows 1 and 3 take it), lane 31 to the rows 2 and 3; the other rows keep `keep`
+__device__ __forceinline__ int lp_row15(int keep, int x) { return __builtin_amdgcn_update_dpp(keep, x, 0x142, 0xa, 0xf, false); }
+__device__ __forceinline__ int lp_row31(int keep, int x) { return __builtin_amdgcn_update_dpp(keep, x, 0x143, 0xc, 0xf, false); }
+__device__ __forceinline__ float lp_row15(float keep, float x) { return __int_as_float(lp_row15(__float_as_int(keep), __float_as_int(x))); }
+__device__ __forceinline__ float lp_row31(float keep, float x) { return __int_as_float(lp_row31(__float_as_int(keep), __float_as_int(x))); }
+__device__ __forceinline__ float lp_lane(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
+__device__ __forceinline__ int lp_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
 
-// over groups of L = 16 or 64 lanes, the result in all of them
-template <int L> __device__ __forceinline__ float lp_max(float x)
+// over groups of L = 16 or 64 lanes, the result in all of them; `none` is the operation's neutral element
+template <int L, class T, class F> __device__ __forceinline__ T lp_reduce(T x, T none, F&& f)
 {
-    x = fmaxf(x, lp_dpp<ROR + 8>(x));
-    x = fmaxf(x, lp_dpp<ROR + 4>(x));
-    x = fmaxf(x, lp_dpp<ROR + 2>(x));
-    x = fmaxf(x, lp_dpp<ROR + 1>(x));
+    x = f(x, lp_dpp<ROR + 8>(x));
+    x = f(x, lp_dpp<ROR + 4>(x));
+    x = f(x, lp_dpp<ROR + 2>(x));
+    x = f(x, lp_dpp<ROR + 1>(x));
     if constexpr (L == 64) {
-        x = fmaxf(x, __shfl_xor(x, 16));
-        x = fmaxf(x, __shfl_xor(x, 32));
+        x = f(x, lp_row15(none, x));
+        x = f(x, lp_row31(none, x));
+        x = lp_lane(x, 63);
     }
     return x;
 }
+template <int L> __device__ __forceinline__ float lp_max(float x)
+{
+    return lp_reduce<L>(x, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
 template <int L> __device__ __forceinline__ float lp_sum(float x)
 {
-    x += lp_dpp<ROR + 8>(x);
-    x += lp_dpp<ROR + 4>(x);
-    x += lp_dpp<ROR + 2>(x);
-    x += lp_dpp<ROR + 1>(x);
+    return lp_reduce<L>(x, 0.0f, [](float a, float b) { return a + b; });
+}
+template <int L> __device__ __forceinline__ int lp_count(int n)
+{
+    return lp_reduce<L>(n, 0, [](int a, int b) { return a + b; });
+}
+
+// the sum of n over the lanes of a group before this one
+template <int L> __device__ __forceinline__ int lp_before_me(int n)
+{
+    int upto = n;
+    upto += lp_dpp<SHR + 1>(upto);
+    upto += lp_dpp<SHR + 2>(upto);
+    upto += lp_dpp<SHR + 4>(upto);
+    upto += lp_dpp<SHR + 8>(upto);
     if constexpr (L == 64) {
-        x += __shfl_xor(x, 16);
-        x += __shfl_xor(x, 32);
+        upto += lp_row15(0, upto);
+        upto += lp_row31(0, upto);
     }
-    return x;
+    return upto - n;
 }
 
 // the statistics of all lanes' columns together
@@ -130,7 +154,7 @@ template <int L> __device__ __forceinline__ float lp_threshold(float lane_max, i
         s = __builtin_amdgcn_fmed3f(s, __shfl_xor(s, 16), b4);
         merge16();
     }
-    return fmaxf(__shfl(s, (lane & (64 - L)) + top - 1), -FLT_MAX);
+    return fmaxf(L == 64 ? lp_lane(s, top - 1) : __shfl(s, (lane & (64 - L)) + top - 1), -FLT_MAX);
 }
 
 // bit (N - 1 - k) for x[k] >= t: bits = 2 bits + (x[k] >= t), a compare and an add with its carry.  The carry may be read two
@@ -161,19 +185,6 @@ __device__ __forceinline__ void lp_mask4(float& x0, float& x1, float& x2, float&
         "v_cndmask_b32 %3, %10, %3, %7"
         : "+v"(x0), "+v"(x1), "+v"(x2), "+v"(x3), "=&s"(a), "=&s"(b), "=&s"(c), "=&s"(d)
         : "v"(ok), "v"(0u), "v"(-INFINITY));
-}
-
-template <int L> __device__ __forceinline__ int lp_count(int n)
-{
-    n += lp_dpp<ROR + 8>(n);
-    n += lp_dpp<ROR + 4>(n);
-    n += lp_dpp<ROR + 2>(n);
-    n += lp_dpp<ROR + 1>(n);
-    if constexpr (L == 64) {
-        n += __shfl_xor(n, 16);
-        n += __shfl_xor(n, 32);
-    }
-    return n;
 }
 
 // floats as integers of the same order, and back
@@ -223,20 +234,7 @@ template <int L, int V, int N> __device__ __forceinline__ unsigned lp_candidates
             }
         }
     }
-    if constexpr (L == 64) count = __builtin_amdgcn_readfirstlane(count);
     return bits;
-}
-
-// the sum of n over the lanes of a group before this one
-template <int L> __device__ __forceinline__ int lp_before_me(int n, int sub)
-{
-    int upto = n;
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) {
-        const int other = __shfl_up(upto, d, L);
-        upto += sub >= d ? other : 0;
-    }
-    return upto - n;
 }
 
 // (v, i) comes before (w, j): larger logit, then lower column
@@ -255,8 +253,8 @@ template <int L> __device__ __forceinline__ int lp_rank(float v, int i, int coun
     if constexpr (L == 16) return lp_rank16(v, i, std::make_integer_sequence<int, 15>());
     int rank = 0;
     for (int k = 0; k < count; k++) {
-        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k));
-        const int j = __builtin_amdgcn_readlane(i, k);
+        const float w = lp_lane(v, k);
+        const int j = lp_lane(i, k);
         rank += lp_before(w, j, v, i);
     }
     return rank;
@@ -272,8 +270,8 @@ __device__ __forceinline__ void lp_insert(LpList& t, float cv, int ci, int lane)
 {
     const unsigned long long before = __ballot(lp_before(t.v, t.i, cv, ci));
     const int pos = __popcll(before);
-    const float sv = __shfl_up(t.v, 1);
-    const int si = __shfl_up(t.i, 1);
+    const float sv = lp_dpp<WAVE_SHR1>(t.v);
+    const int si = lp_dpp<WAVE_SHR1>(t.i);
     if (lane == pos) { t.v = cv; t.i = ci; }
     else if (lane > pos) { t.v = sv; t.i = si; }
 }
@@ -397,7 +395,7 @@ template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_b
         for (int k = 0; k < N; k++) mine_x[k] = x[k];
         int count;
         unsigned bits = lp_candidates<L, V>(x, lane_max, s.m, A.top, lane, count);
-        int at = group + lp_before_me<L>(__popc(bits), sub);
+        int at = group + lp_before_me<L>(__popc(bits));
         lp_wave_sync();
         while (__any(bits != 0)) {
             if (bits) {
@@ -509,7 +507,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
                         while (better) {
                             const int src = __ffsll((long long)better) - 1;
                             better &= better - 1;
-                            lp_insert(t, __shfl(x[k], src), min(base + ((k / V) * 64 + src) * V, last) + k % V, lane);
+                            lp_insert(t, lp_lane(x[k], src), min(base + ((k / V) * 64 + src) * V, last) + k % V, lane);
                         }
                     }
                 } else {
@@ -517,7 +515,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
                     int* wi = lds_i + wave * 64;
                     int count;
                     const unsigned enter = lp_candidates<64, V>(x, lane_max, lp_max<64>(lane_max), A.top, lane, count);
-                    int at = lp_before_me<64>(__popc(enter), lane);
+                    int at = lp_before_me<64>(__popc(enter));
 #pragma unroll
                     for (int k = 0; k < LP_E; k++)
                         if (enter & (1u << (LP_E - 1 - k))) {
@@ -542,8 +540,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
                         lp_wave_sync();
                         int before = 0;
                         for (int k = 0; k < count; k++) {
-                            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k));
-                            const int j = __builtin_amdgcn_readlane(i, k);
+                            const float w = lp_lane(v, k);
+                            const int j = lp_lane(i, k);
                             before += lp_before(w, j, t.v, t.i);
                         }
                         if (lane + before < 64) {
@@ -561,7 +559,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
                     t.i = wi[lane];
                     lp_wave_sync();
                 }
-                worst = __shfl(t.v, A.top - 1);
+                worst = lp_lane(t.v, A.top - 1);
             }
         }
     }
@@ -645,12 +643,12 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs A, int splits, con
         const float T = lp_threshold<64>(lane < splits ? lds_v[lane * top + j] : -INFINITY, r, lane);
         // entries of this lane's list that come before (t, i)
         const auto reach = [&](float t, int i) { return lane < splits ? lp_search(lds_v + lane * top, lds_i + lane * top, top, t, i) : 0; };
-        int mine = reach(T, LP_NONE), count = __builtin_amdgcn_readfirstlane(lp_count<64>(mine));      // those that are >= T
+        int mine = reach(T, LP_NONE), count = lp_count<64>(mine);      // those that are >= T
         if (count > 64) {                                  // halved as in lp_candidates: values, then columns of one value
             const auto halve = [&](int lo, int hi, auto&& before) {
                 while (count > 64 && (unsigned)hi - (unsigned)lo > 1u) {
                     const int mid = __builtin_amdgcn_readfirstlane((int)((unsigned)lo + (((unsigned)hi - (unsigned)lo) >> 1)));
-                    const int m = before(mid), n = __builtin_amdgcn_readfirstlane(lp_count<64>(m));
+                    const int m = before(mid), n = lp_count<64>(m);
                     if (n >= top) {
                         lo = mid;
                         mine = m;
@@ -663,7 +661,7 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs A, int splits, con
                                  [&](int mid) { return reach(__int_as_float(lp_key(mid)), LP_NONE); });
             halve(-LP_NONE, 0, [&](int mid) { return reach(__int_as_float(lp_key(lo)), -mid); });      // (the fewer, the larger mid)
         }
-        const int at = lp_before_me<64>(mine, lane);
+        const int at = lp_before_me<64>(mine);
         for (int k = 0; k < mine; k++) {
             cand_v[at + k] = lds_v[lane * top + k];
             cand_i[at + k] = lds_i[lane * top + k];
