@@ -212,6 +212,10 @@ class Context:
             return None
         if not torch.is_tensor(x):
             x = torch.as_tensor(x)
+        if dtype is torch.int32 and x.dtype is not dtype:
+            if x.is_floating_point() or x.dtype is torch.bool:
+                raise ValueError(f"{what}: integers, got {x.dtype}")
+            x = x.clamp(min=-1, max=0x7fffffff) if x.dtype is torch.int64 else x       # (out of range stays out of range)
         if x.dtype is not dtype or x.device != self.device or not x.is_contiguous():
             x = x.to(self.device, dtype=dtype).contiguous()
         if x.numel() != rows:

@@ -360,6 +360,47 @@ def test_two_streams_and_a_graph():
     two.close()
 
 
+@pytest.mark.parametrize("rows,cols", [(67_200_003, 3), (4_194_310, 1025)])
+def test_more_rows_than_one_launch_takes(ctx, rows, cols):
+    x = torch.zeros((rows, cols), dtype=torch.float16, device="cuda")
+    far = torch.randn(20, cols).half().cuda()
+    x[-20:] = far
+    a = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    a[-20:] = torch.arange(20).cuda() % cols
+    r = ctx.action_logprobs(x, a, top=2)
+    want = definition(far, None, a[-20:], 1.0, 2)
+    lse, ent, lp = bounds(want, cols)
+    same(r.logp[-20:], want["logp"], lp(want["logp"]))
+    same(r.lse[-20:], want["lse"], lse)
+    same(r.entropy[-20:], want["entropy"], ent)
+    assert np.array_equal(r.top_actions[-20:].cpu().numpy(), want["top_actions"])
+    head = r.lse[:-20]
+    assert (head - math.log(cols)).abs().max() <= 64 * U * (1 + math.log(cols)) and (r.top_actions[:-20] == torch.arange(2).cuda()).all()
+    g = torch.ones(rows, device="cuda")
+    d = ctx.action_logprobs_grad(x, a, r.lse, r.entropy, g, None)
+    p = torch.from_numpy(want["p"])
+    hot = torch.nn.functional.one_hot(a[-20:].long().cpu(), cols)
+    assert (d[-20:].double().cpu() - (hot - p)).abs().max() <= 2.0 ** -11 + 1e-5
+    assert (d[:-20, 0].float() - (1 - 1 / cols)).abs().max() <= 2.0 ** -11 + 1e-5
+    assert (d[:-20, 1:].float() + 1 / cols).abs().max() <= 2.0 ** -11 / cols + 2.0 ** -24
+
+
+def test_mask_bytes_and_action_types(ctx):
+    """Any byte but 0 allows; actions of other integer types, values beyond 32 bits included, mean what they say."""
+    x, valid, a = make(9, 82, torch.float32, 2, True)
+    want = ctx.action_logprobs(x, a, valid=valid, top=4)
+    for scaled in (valid * 255, valid * 128, valid.bool(), valid * torch.arange(1, 83, dtype=torch.uint8).cuda()):
+        got = ctx.action_logprobs(x, a, valid=scaled, top=4)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    assert all(torch.equal(p, q) for p, q in zip(ctx.action_logprobs(x, a.long(), valid=valid, top=4), want))
+    far = torch.tensor([2 ** 32 + 5, -2 ** 33, 3]).cuda()
+    r = ctx.action_logprobs(x[:3], far)
+    assert torch.isnan(r.logp[0]) and float(r.logp[1]) == 0.0 and float(r.logp[2]) < 0
+    for bad in (torch.ones(9), torch.ones(9, dtype=torch.bool)):
+        with pytest.raises(ValueError, match="integers"):
+            ctx.action_logprobs(x, bad.cuda())
+
+
 def test_same_bits_twice(ctx):
     for rows, cols in ((50, 362), (4, 150_001), (300, 9001)):
         x, valid, a = make(rows, cols, torch.bfloat16, 3, True)
