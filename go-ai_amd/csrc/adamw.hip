@@ -65,9 +65,10 @@ struct goai_adamw {
     goai::AwState state{};
     std::vector<goai::AwTensor> tensors;
     std::vector<int> first;                    // first chunk of each tensor (and the total)
+    char* d_mem = nullptr;                     // one allocation: the norm's partial sums, tensors, chunks
+    double* d_partials = nullptr;              // AW_NORM_BLOCKS
     goai::AwTensor* d_tensors = nullptr;
     goai::AwChunk* d_chunks = nullptr;
-    double* d_partials = nullptr;              // AW_NORM_BLOCKS
 };
 
 namespace goai {
@@ -361,23 +362,26 @@ __global__ __launch_bounds__(256) void k_adamw_norm(const double* __restrict__ p
     }
 }
 
-// ---- 8-bit moments from and to float32 arrays of the same layout ----
-__global__ __launch_bounds__(256) void k_adamw_pack(const AwTensor* __restrict__ tensors, const AwChunk* __restrict__ chunks, AwState S,
-                                                    const float* __restrict__ m_in, const float* __restrict__ v_in)
+// ---- one of the moments (ROOT: the second) from float32 tensors, 8-bit ones to a float32 array of the flat layout ----
+template <int BITS, bool ROOT>
+__global__ __launch_bounds__(256) void k_adamw_load(const AwTensor* __restrict__ tensors, const AwChunk* __restrict__ chunks, int base, AwState S,
+                                                    AwGrads from)
 {
     const AwChunk ch = chunks[blockIdx.x];
     const AwTensor T = tensors[ch.tensor];
     const long i = (long)ch.chunk * AW_CHUNK + threadIdx.x * 8, j = T.start + i;
     if (i / AW_BLOCK * AW_BLOCK >= T.n) return;
-    float m[8], v[8], root[8], ms, vs;
-    aw_load<0>(m_in + T.start, i, T.n, m);
-    aw_load<0>(v_in + T.start, i, T.n, v);
-    aw_sqrt(v, root);
-    *(AwCodes*)((char*)S.m + j) = aw_pack_mean(m, ms);
-    *(AwCodes*)((char*)S.v + j) = aw_pack_root(root, vs);
-    if (j % AW_BLOCK == 0) {
-        S.ms[j / AW_BLOCK] = ms;
-        S.vs[j / AW_BLOCK] = vs;
+    float x[8];
+    aw_load<0>(from.g[ch.tensor - base], i, T.n, x);
+    if constexpr (BITS == 32) aw_store<0>((float*)(ROOT ? S.v : S.m) + T.start, i, T.n, x);
+    else {
+        float scale;
+        if constexpr (ROOT) {
+            float r[8];
+            aw_sqrt(x, r);
+            *(AwCodes*)((char*)S.v + j) = aw_pack_root(r, scale);
+        } else *(AwCodes*)((char*)S.m + j) = aw_pack_mean(x, scale);
+        if (j % AW_BLOCK == 0) (ROOT ? S.vs : S.ms)[j / AW_BLOCK] = scale;
     }
 }
 
@@ -407,9 +411,7 @@ int64_t adamw_state_elems(int n, const int64_t* numels)
 static void aw_free(goai_adamw* o)
 {
     if (!o) return;
-    (void)hipFree(o->d_tensors);
-    (void)hipFree(o->d_chunks);
-    (void)hipFree(o->d_partials);
+    (void)hipFree(o->d_mem);
     delete o;
 }
 
@@ -451,12 +453,15 @@ static int aw_build(goai_adamw* o, int n, void* const* params, const int32_t* pt
         o->elems += aw_padded(numels[i]);
     }
     o->first.push_back((int)chunks.size());
-    const size_t tb = o->tensors.size() * sizeof(AwTensor), cb = std::max<size_t>(chunks.size(), 1) * sizeof(AwChunk);
-    GOAI_HIP_CHECK(hipMalloc((void**)&o->d_tensors, tb));
-    GOAI_HIP_CHECK(hipMalloc((void**)&o->d_chunks, cb));
-    GOAI_HIP_CHECK(hipMalloc((void**)&o->d_partials, AW_NORM_BLOCKS * sizeof(double)));
-    GOAI_HIP_CHECK(hipMemcpy(o->d_tensors, o->tensors.data(), tb, hipMemcpyHostToDevice));
-    if (!chunks.empty()) GOAI_HIP_CHECK(hipMemcpy(o->d_chunks, chunks.data(), chunks.size() * sizeof(AwChunk), hipMemcpyHostToDevice));
+    const size_t pb = AW_NORM_BLOCKS * sizeof(double), tb = o->tensors.size() * sizeof(AwTensor), cb = chunks.size() * sizeof(AwChunk);
+    std::vector<char> image(pb + tb + cb);
+    memcpy(image.data() + pb, o->tensors.data(), tb);
+    if (cb) memcpy(image.data() + pb + tb, chunks.data(), cb);
+    GOAI_HIP_CHECK(hipMalloc((void**)&o->d_mem, image.size()));
+    GOAI_HIP_CHECK(hipMemcpy(o->d_mem, image.data(), image.size(), hipMemcpyHostToDevice));
+    o->d_partials = (double*)o->d_mem;
+    o->d_tensors = (AwTensor*)(o->d_mem + pb);
+    o->d_chunks = (AwChunk*)(o->d_mem + pb + tb);
     return GOAI_OK;
 }
 
@@ -556,17 +561,21 @@ int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, 
     });
 }
 
-int adamw_load_moments(goai_ctx* c, goai_adamw* o, const float* m, const float* v)
+int adamw_load_moments(goai_ctx* c, goai_adamw* o, const float* const* m, const float* const* v)
 {
     GOAI_REQUIRE(o->device == c->device, "adamw: the optimiser lives on another GPU");
-    if (o->bits == 32) {
-        GOAI_HIP_CHECK(hipMemcpyAsync(o->state.m, m, o->elems * sizeof(float), hipMemcpyDeviceToDevice, c->stream));
-        GOAI_HIP_CHECK(hipMemcpyAsync(o->state.v, v, o->elems * sizeof(float), hipMemcpyDeviceToDevice, c->stream));
-        return GOAI_OK;
+    for (size_t i = 0; i < o->tensors.size(); i++) {
+        GOAI_REQUIRE(o->tensors[i].n == 0 || (m[i] && v[i]), "adamw: NULL moment");
+        GOAI_REQUIRE((((uintptr_t)m[i] | (uintptr_t)v[i]) & 3) == 0, "adamw: a moment is not aligned to its element type");
     }
-    if (o->first.back()) k_adamw_pack<<<o->first.back(), 256, 0, c->stream>>>(o->d_tensors, o->d_chunks, o->state, m, v);
-    GOAI_HIP_CHECK(hipGetLastError());
-    return GOAI_OK;
+    const auto load = [&](const float* const* from, auto kernel) {
+        return aw_launches(o, (const void* const*)from, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
+            if (n) kernel<<<n, 256, 0, c->stream>>>(o->d_tensors, chunks, base, o->state, g);
+        });
+    };
+    const int rc = o->bits == 8 ? load(m, k_adamw_load<8, false>) : load(m, k_adamw_load<32, false>);
+    if (rc) return rc;
+    return o->bits == 8 ? load(v, k_adamw_load<8, true>) : load(v, k_adamw_load<32, true>);
 }
 
 int adamw_moments(goai_ctx* c, goai_adamw* o, float* m, float* v)

@@ -626,7 +626,7 @@ int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, in
     return adamw_step(ctx, opt, grads, t, lr, beta1, beta2, eps, max_norm, norm_and_coef, scalars);
 }
 
-int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* exp_avg, const float* exp_avg_sq)
+int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* const* exp_avg, const float* const* exp_avg_sq)
 {
     GOAI_REQUIRE(opt && exp_avg && exp_avg_sq, "NULL argument");
     CTX_ENTER(ctx);

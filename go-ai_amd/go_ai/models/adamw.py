@@ -201,14 +201,14 @@ class AdamW:
         for a, b, s in zip(exp_avg, exp_avg_sq, self._shapes):
             if a.shape != s or b.shape != s:
                 raise ValueError(f"AdamW: a parameter of shape {tuple(s)}, moments of shapes {tuple(a.shape)} and {tuple(b.shape)}")
-        flat = (self._m, self._v)
-        if self.state_bits == 8:
-            flat = [torch.zeros(self._elems, dtype=torch.float32, device=self.device) for _ in range(2)]
-        for to, given in zip(flat, (exp_avg, exp_avg_sq)):
-            torch._foreach_copy_(self._split(to), list(given))
-        if self.state_bits == 8 and self._elems:
-            from .. import _hip
-            _hip.check(_hip.lib.goai_adamw_load_moments(self._ctx._h, self._h, flat[0].data_ptr(), flat[1].data_ptr()))
+        from .. import _hip
+        tables, held = [], []
+        for given in (exp_avg, exp_avg_sq):
+            given = [x if x.dtype is torch.float32 and x.device == self.device and x.is_contiguous()
+                     else x.to(self.device, dtype=torch.float32).contiguous() for x in given]
+            held.append(given)
+            tables.append(_ctypes_table(ctypes.c_void_p, list(map(_address_of, given))))
+        _hip.check(_hip.lib.goai_adamw_load_moments(self._ctx._h, self._h, *tables))
         self.steps = int(steps)
 
     def state_dict(self):

@@ -481,8 +481,9 @@ int goai_adamw_grad_norm(goai_ctx* ctx, goai_adamw* opt, const void* const* grad
 int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, int64_t t, double lr, double beta1, double beta2,
                     double eps, double max_norm, float* norm_and_coef, const double* scalars);
 
-/* Moments from / to float32 arrays [elems] of the flat layout (16-byte aligned), rounding to / reading the 8-bit codes. */
-int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* exp_avg, const float* exp_avg_sq);
+/* Moments from float32 tensors (HOST tables of DEVICE pointers in the tensors' order; 8-bit ones are rounded to their codes). */
+int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* const* exp_avg, const float* const* exp_avg_sq);
+/* Moments to float32 arrays [elems] of the flat layout (16-byte aligned): the values that 8-bit codes stand for. */
 int goai_adamw_moments(goai_ctx* ctx, goai_adamw* opt, float* exp_avg, float* exp_avg_sq);
 
 /* ---------------------------------------------------------------------------------------
