@@ -89,8 +89,8 @@ extern "C" int goai_debug_wino2s_stamps(unsigned long long* host_out, int n)
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned w2s_v4u __attribute__((vector_size(16)));
-// y -= m as two v_pk_fma_f32 by n1 = (-1, -1), a value the optimiser cannot see through: it turns a plain vector
-// subtraction (and a multiply-add by a visible -1.0) into four v_sub_f32 -- twice the issue slots.  fma(m, -1, y) = y - m exactly.
+// y -= m as fma(m, n1, y) with n1 = (-1, -1): y - m exactly.  (Written in pairs when the library was built with packed fp32
+// instructions, where a plain subtraction took twice the issue slots; without them, as now, both are four instructions.)
 __device__ __forceinline__ void w2s_sub4(f32x4& y, const f32x4 m, const f32x2 n1)
 {
     const f32x2 lo = __builtin_elementwise_fma(__builtin_shufflevector(m, m, 0, 1), n1, __builtin_shufflevector(y, y, 0, 1));

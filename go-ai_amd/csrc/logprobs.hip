@@ -51,8 +51,8 @@ __device__ __forceinline__ void lp_raise(LpStat& s, float m, LpFactor c)     // 
     s.m = m;
 }
 
-// ---- cross-lane helpers: DPP moves within rows of 16 lanes and from row to row (no LDS unit: some 8 cycles a step against
-// some 100 of a shuffle) ----
+// ---- cross-lane helpers: DPP moves within rows of 16 lanes and from row to row, which do without the LDS unit that shuffles go
+// through (5 x 128001 rising columns, 20 alternatives: 27 -> 24 us a call) ----
 template <int CTRL> __device__ __forceinline__ int lp_dpp(int x) { return __builtin_amdgcn_mov_dpp(x, CTRL, 0xf, 0xf, true); }
 template <int CTRL> __device__ __forceinline__ float lp_dpp(float x) { return __int_as_float(lp_dpp<CTRL>(__float_as_int(x))); }
 constexpr int SHR = 0x110, ROR = 0x120, WAVE_SHR1 = 0x138, MIRROR = 0x140, HALF_MIRROR = 0x141, XOR1 = 0xb1, XOR2 = 0x4e, XOR3 = 0x1b;
@@ -422,7 +422,9 @@ template <int E, int L, int V, int NV, int FULL, bool TOP> __global__ __launch_b
 // tile's, and those of rows that rise -- as a list of the tile's own that is merged in.
 constexpr int LP_E = 16;                                   // columns per lane and tile
 constexpr int LP_TILE = 64 * LP_E;
-constexpr int LP_FEW = 12;                                 // columns that enter a list one by one: some 60 cycles each, a list of their own 800
+// columns that enter a list one by one, more as a list of their own (1500 x 50021 float32, 20 alternatives: with 4 98 us, 12 71, 24 66,
+// 48 67; 20000 x 2000: 60, 60, 52, 52)
+constexpr int LP_FEW = 24;
 constexpr int LP_SPLITS = 64;                              // at most: one list per lane when they are joined
 
 struct LpPart {                                            // a segment's result in the workspace
@@ -463,7 +465,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
     float worst = -INFINITY;                               // the last alternative of the tiles before
     for (int base = c0 + (W == 4 ? wave : 0) * LP_TILE; base < c1; base += W * LP_TILE) {
         // the loads are issued before the first is used; a vector that would pass the row's end starts V columns before it, and its
-        // columns in front of the lane's own are another lane's (rows of this kernel are longer than a tile)
+        // columns in front of the lane's own are another lane's (rows of this kernel are longer than a vector)
         float x[LP_E];
         {
             ElemVec<E, V> u[NV];
@@ -763,15 +765,15 @@ static LpFactor lp_factor(double c)
         default: { constexpr int E = 2; __VA_ARGS__; } break;        \
     }
 
-constexpr int LP_SHORT = 1024;                      // longest row that stays in a wavefront's registers
+constexpr int LP_SHORT = 384;                       // longest row that stays in registers (30000 x 1000 float32: 28 us there, 23 below)
 
 // Long rows: from LP_MANY rows on they fill the GPU a wavefront each (20000 x 2000 float32, 5 alternatives: 40 us, with four wavefronts a
 // row 85; 2048 x 40000: 67 and 70; 1024 x 40000: 56 and 37); fewer rows take four wavefronts a segment, in as many segments as fill
-// it.  A segment is a multiple of four tiles, one for each.
-constexpr int64_t LP_MANY = 2048;
+// it (LP_FILL; 5 x 128001: 18.5 us, with 256 21.4; 700 x 8000: 15 us, with 1024, which splits the rows, 18).  A segment is a multiple of four tiles, one for each.
+constexpr int64_t LP_MANY = 2048, LP_FILL = 512;
 static int lp_segment(int64_t rows, int cols)
 {
-    const int64_t want = std::min<int64_t>((512 + rows - 1) / rows, LP_SPLITS), unit = 4 * LP_TILE;
+    const int64_t want = std::min<int64_t>((LP_FILL + rows - 1) / rows, LP_SPLITS), unit = 4 * LP_TILE;
     return (int)(((cols + want - 1) / want + unit - 1) / unit * unit);
 }
 static int lp_splits(int64_t rows, int cols) { return cols <= LP_SHORT ? 1 : (cols - 1) / lp_segment(rows, cols) + 1; }
@@ -815,9 +817,9 @@ template <int E, int L, int V, int NV, int FULL> static void lp_launch_short(con
 
 template <int E> static void lp_launch(const LpArgs& A, void* workspace, hipStream_t st)
 {
-    // sixteen lanes per row: up to 384 columns and eight alternatives (of sixteen lanes' maxima the eighth is still a sharp
-    // threshold); else a wavefront per row
-    if (A.cols <= 384 && A.top <= 8) {
+    // sixteen lanes per row: up to eight alternatives (of sixteen lanes' maxima the eighth is still a sharp threshold; 65536 x 362
+    // bfloat16: 21 us, with a wavefront per row 46; 300000 x 82 float32: 48 and 145); more: a wavefront per row
+    if (A.cols <= LP_SHORT && A.top <= 8) {
         if (A.cols <= 32) lp_launch_short<E, 16, 1, 2, 0>(A, st);
         else if (A.cols <= 64) lp_launch_short<E, 16, 4, 1, 0>(A, st);
         else if (A.cols <= 128) lp_launch_short<E, 16, 4, 2, 1>(A, st);
@@ -825,14 +827,13 @@ template <int E> static void lp_launch(const LpArgs& A, void* workspace, hipStre
         else lp_launch_short<E, 16, 4, 6, 3>(A, st);
     } else if (A.cols <= LP_SHORT) {
         if (A.cols <= 128) lp_launch_short<E, 64, 1, 2, 0>(A, st);
-        else if (A.cols <= 384) lp_launch_short<E, 64, 1, 6, 2>(A, st);
-        else lp_launch_short<E, 64, 1, 16, 6>(A, st);
+        else lp_launch_short<E, 64, 1, 6, 2>(A, st);
     } else {
         const int segment = lp_segment(A.rows, A.cols), splits = lp_splits(A.rows, A.cols);
         LpPart* parts = (LpPart*)workspace;
         float* pv = (float*)(parts + A.rows * splits);
         int* pi = (int*)(pv + A.rows * splits * A.top);
-        // (splits > 1 only for fewer than 512 rows: one round)
+        // (splits > 1 only for fewer than LP_FILL rows: one round)
         const bool many = A.rows >= LP_MANY;
         lp_chunks<E>(A, LP_GRID, [&](const LpArgs& B) {
             const unsigned grid = many ? (unsigned)((B.rows + 3) / 4) : (unsigned)(B.rows * splits);
@@ -881,6 +882,7 @@ template <int E> static void lp_launch_grad(const LpGradArgs& A, hipStream_t st)
     constexpr int V = E == 0 ? 4 : 8;                   // 16 bytes; 8 of a short row, which has few vectors for its lanes (300000 x 26
     if (A.cols < 4) lp_launch_grad<E, 16, 1>(A, st);    // bfloat16: 21 us, with 16 bytes 30)
     else if (A.cols <= LG_N * 16 * 4) lp_launch_grad<E, 16, 4>(A, st);
+    // lanes a row: 50000 x 362 bfloat16 20 us with 16, 22 with 64; 30000 x 1500 38 us with 64, 49 with 256
     else if (A.cols <= LG_N * 16 * V) lp_launch_grad<E, 16, V>(A, st);
     else if (A.cols <= LG_N * 64 * V) lp_launch_grad<E, 64, V>(A, st);
     else lp_launch_grad<E, 256, V>(A, st);

@@ -223,7 +223,7 @@ class Context:
         return x
 
     LOGPROBS_MAX_TOP = 64
-    LOGPROBS_SHORT = 1024        # up to so many columns goai_action_logprobs needs no workspace
+    LOGPROBS_SHORT = 4096        # up to so many columns goai_action_logprobs needs no workspace
 
     def action_logprobs(self, logits, actions=None, valid=None, temperature=1.0, top=0):
         """goai_action_logprobs: log probabilities of `actions` [rows] under softmax(logits / temperature) over the columns with

@@ -39,7 +39,7 @@ def test_logprobs(bad, message):
 
 def test_logprobs_workspace():
     f = lib.goai_action_logprobs_workspace
-    assert f(5, 82, 64) == 0 and f(0, 1 << 30, 64) == 0 and f(1, 1024, 64) == 0
+    assert f(5, 82, 64) == 0 and f(0, 1 << 30, 64) == 0 and f(1, 4096, 64) == 0
     for rows in (1, 3, 511, 512, 100_000):
         for cols in (1025, 4097, 70_001, 1 << 30):
             for top in (0, 64):
