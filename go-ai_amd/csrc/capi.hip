@@ -550,6 +550,20 @@ int64_t goai_action_logprobs_workspace(int64_t rows, int cols, int top)
     return action_logprobs_workspace(rows, cols, top);
 }
 
+// Whether two matrices of the same shape and element size share memory without being the same one (rows may lie between each other's,
+// as two column ranges of one array do)
+static bool rows_overlap(const void* x, int64_t xstride, const void* d, int64_t dstride, int64_t rows, int cols, int64_t size)
+{
+    const __int128 x0 = (__int128)(uintptr_t)x, d0 = (__int128)(uintptr_t)d, row = (__int128)cols * size;
+    const auto end = [&](__int128 at, int64_t stride) { return at + (__int128)(rows - 1) * stride * size + row; };
+    if (rows == 0 || end(x0, xstride) <= d0 || end(d0, dstride) <= x0) return false;
+    if (rows == 1) return x0 != d0;
+    if (xstride != dstride) return true;
+    if (x0 == d0) return false;
+    const __int128 step = (__int128)xstride * size, off = ((d0 - x0) % step + step) % step;
+    return off < row || off > step - row;
+}
+
 int goai_action_logprobs_grad(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid, int64_t valid_stride,
                               const int32_t* actions, double temperature, const float* lse, const float* entropy, const float* d_logp,
                               const float* d_entropy, void* d_logits, int64_t d_stride, int64_t rows, int cols)
@@ -561,6 +575,8 @@ int goai_action_logprobs_grad(goai_ctx* ctx, const void* logits, int elem_type, 
     GOAI_REQUIRE(rows == 0 || !d_entropy || entropy, "d_entropy needs entropy");
     GOAI_REQUIRE(d_stride >= cols, "d_stride is smaller than the row");
     GOAI_REQUIRE((uintptr_t)d_logits % (elem_type == GOAI_ELEM_F32 ? 4 : 2) == 0, "d_logits is not aligned to its element type");
+    GOAI_REQUIRE(!rows_overlap(logits, row_stride, d_logits, d_stride, rows, cols, elem_type == GOAI_ELEM_F32 ? 4 : 2),
+                 "d_logits overlaps the logits without being them");
     CTX_ENTER(ctx);
     if (rows == 0) return GOAI_OK;
     return launch_action_logprobs_grad(logits, elem_type, row_stride, valid, valid_stride, actions, temperature, lse, entropy, d_logp, d_entropy,

@@ -269,8 +269,6 @@ class Context:
         elif (out.dtype != x.dtype or tuple(out.shape) != (rows, cols) or out.device != self.device
               or (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols)):
             raise ValueError("out: a matrix of the logits' shape, type and device, its columns next to each other")
-        elif out.data_ptr() == x.data_ptr() and rows > 1 and out.stride(0) != xs:
-            raise ValueError("out: the logits themselves, or memory of its own")
         if rows:
             p = _hip.dptr
             _hip.check(_hip.lib.goai_action_logprobs_grad(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), temperature, p(l), p(e), p(g),

@@ -435,7 +435,8 @@ int64_t goai_action_logprobs_workspace(int64_t rows, int cols, int top);
  *   d_logits[i][j] = (d_logp (delta(actions[i], j) - p_j) - d_entropy p_j (log p_j + entropy)) / temperature
  * on allowed columns, 0 on the others; in the logits' type.  lse and entropy (needed with d_entropy) are goai_action_logprobs'
  * outputs for the same logits, mask and temperature.  A row whose actions[i] < 0 has no d_logp term; actions[i] >= cols
- * makes the row NaN.  d_logits may be the logits themselves when d_stride == row_stride; otherwise they must not overlap. */
+ * makes the row NaN.  d_logits may be the logits themselves when d_stride == row_stride, or another column range of the same array;
+ * any other overlap is refused. */
 int goai_action_logprobs_grad(goai_ctx* ctx, const void* logits, int elem_type, int64_t row_stride, const uint8_t* valid,
                               int64_t valid_stride, const int32_t* actions, double temperature, const float* lse,
                               const float* entropy, const float* d_logp, const float* d_entropy, void* d_logits, int64_t d_stride,

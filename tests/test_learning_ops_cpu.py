@@ -59,6 +59,14 @@ def grad(**k):
     (dict(), "ctx is NULL"), (dict(lse=None), "lse"), (dict(d=None), "d_logits"), (dict(actions=None), "actions"), (dict(ent=None), "entropy"),
     (dict(ds=81), "d_stride"), (dict(ds=0), "d_stride"), (dict(d=66), "aligned"), (dict(t=0.0), "temperature"), (dict(logits=None), "logits"),
     (dict(ent=None, h=None), "ctx is NULL"), (dict(actions=None, g=None), "ctx is NULL"),
+    # the logits at 1000 (4 rows of 82 float32) and a gradient that is on, beside or between them
+    (dict(logits=1000, d=1000), "ctx is NULL"), (dict(logits=1000, d=1004), "overlaps"), (dict(logits=1004, d=1000), "overlaps"),
+    (dict(logits=1000, d=1000, ds=83), "overlaps"), (dict(logits=1000, d=1000, stride=0), "overlaps"),
+    (dict(logits=1000, d=1000 + 4 * 328), "ctx is NULL"), (dict(logits=1000 + 4 * 328, d=1000), "ctx is NULL"),
+    (dict(logits=1000, d=996 + 4 * 328), "overlaps"), (dict(logits=1000, d=1000 + 4 * 82), "overlaps"),
+    (dict(logits=1000, d=1000 + 4 * 82, stride=164, ds=164), "ctx is NULL"), (dict(logits=1000 + 4 * 82, d=1000, stride=164, ds=164), "ctx is NULL"),
+    (dict(logits=1000, d=996 + 4 * 82, stride=164, ds=164), "overlaps"), (dict(logits=1000, d=1004 + 4 * 82, stride=164, ds=164), "overlaps"),
+    (dict(logits=1000, d=1000, rows=1, stride=90), "ctx is NULL"), (dict(logits=1000, d=1004, rows=1), "overlaps"),
 ])
 def test_gradient(bad, message):
     assert grad(**bad) == -1 and message in err()
