@@ -167,6 +167,7 @@ int train_load(goai_ctx* c, const char* const* names, const float* const* tensor
     GOAI_REQUIRE(t.ready, "call goai_train_init first");
     GOAI_REQUIRE(names && tensors && numels && n > 0, "NULL / empty weight table");
     GOAI_HIP_CHECK(hipStreamSynchronize(c->stream));
+    t.actor_rows = 0;                              // (its activations were other parameters')
     size_t seen = 0;
     for (int i = 0; i < n; i++) {
         GOAI_REQUIRE(names[i] && tensors[i], "NULL entry in weight table");

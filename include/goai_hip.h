@@ -382,7 +382,7 @@ int goai_train_backward(goai_ctx* ctx, const uint8_t* states, const uint8_t* nex
 /* The actor alone, for losses of the caller's own (actor-critic net): its logits [n][A] of n positions in training mode (BatchNorm on
  * the batch's statistics, the running ones move), and from the loss's gradient with respect to them all parameters' gradients
  * (0 for the critic's head) in the flat buffer of goai_train_grads.  The backward call follows its forward call on the
- * same context with no training call in between (else GOAI_ERR_STATE).  2 <= n <= max_batch.  Asynchronous. */
+ * same context with no step, backward or load call in between (else GOAI_ERR_STATE).  2 <= n <= max_batch.  Asynchronous. */
 int goai_train_actor_forward(goai_ctx* ctx, const uint8_t* states, float* logits, int n);
 int goai_train_actor_backward(goai_ctx* ctx, const float* d_logits, int n);
 

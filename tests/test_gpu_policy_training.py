@@ -251,3 +251,16 @@ def test_move_logprobs(size):
     assert np.array_equal(r.top_actions.cpu().numpy(), np.where(there, order, -1))
     assert np.abs(r.top_logp.cpu().numpy()[there] - best[there]).max() <= tol
     assert net.move_logprobs(states).logp is None
+
+
+def test_loaded_parameters_end_an_actor_pass():
+    from go_ai import _hip
+    from go_ai.engine import Context
+    c = Context(5)
+    c.train_init(Context.NET_AC, 1, 8)
+    sd = nn_ref.make_state_dict("ac", 5, 1, layers=1)
+    c.train_load(sd)
+    c.train_actor_forward(np.zeros((3, 6, 5, 5), np.uint8))
+    c.train_load(sd)
+    with pytest.raises(_hip.GoaiError, match="must follow"):
+        c.train_actor_backward(torch.zeros(3, 26).cuda())
