@@ -30,6 +30,7 @@ def _dev_u8_states(states, device):
 
 
 ELEM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # GOAI_ELEM_*
+INTEGER_TYPES = {torch.int8, torch.uint8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64}
 
 # what Context.action_logprobs returns: float32 [rows] (logp None without actions) and [rows, top] (None for top = 0)
 ActionLogprobs = collections.namedtuple("ActionLogprobs", "logp entropy lse top_actions top_logp")
@@ -213,9 +214,10 @@ class Context:
         if not torch.is_tensor(x):
             x = torch.as_tensor(x)
         if dtype is torch.int32 and x.dtype is not dtype:
-            if x.is_floating_point() or x.dtype is torch.bool:
-                raise ValueError(f"{what}: integers, got {x.dtype}")
-            x = x.clamp(min=-1, max=0x7fffffff) if x.dtype is torch.int64 else x       # (out of range stays out of range)
+            if x.dtype not in INTEGER_TYPES:
+                raise ValueError(f"{what}: signed integers or up to 32 bits, got {x.dtype}")
+            if x.dtype in (torch.int64, torch.uint32):
+                x = x.to(torch.int64).clamp(min=-1, max=0x7fffffff)                    # (out of range stays out of range)
         if x.dtype is not dtype or x.device != self.device or not x.is_contiguous():
             x = x.to(self.device, dtype=dtype).contiguous()
         if x.numel() != rows:

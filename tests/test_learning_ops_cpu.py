@@ -130,3 +130,20 @@ def test_adamw_without_a_gpu_is_only_numbers():
     for bad in (dict(lr=-1), dict(betas=(0.9, 1.0)), dict(eps=0), dict(state_bits=4), dict(max_norm=-1)):
         with pytest.raises(ValueError):
             AdamW(None, **bad)
+
+
+@pytest.mark.parametrize("dtype", ["int8", "uint8", "int16", "uint16", "int32", "uint32", "int64", "uint64", "float32", "bool", "complex64"])
+def test_action_types(dtype):
+    """Actions of every integer type mean what they say, or are refused: the largest of a type is not -1 (no action)."""
+    import torch
+    from go_ai.engine import Context
+    c = object.__new__(Context)
+    c._h, c.device = None, torch.device("cpu")
+    kind = np.dtype(dtype)
+    if kind.kind not in "iu" or dtype == "uint64":
+        with pytest.raises(ValueError, match="actions"):
+            c._per_row(np.zeros(2, kind), 2, torch.int32, "actions")
+        return
+    least, most = np.iinfo(kind).min, np.iinfo(kind).max
+    got = c._per_row(np.array([least, 5, most], kind), 3, torch.int32, "actions").tolist()
+    assert got == [max(least, -1) if kind.itemsize == 8 else least, 5, min(most, 0x7fffffff)]
