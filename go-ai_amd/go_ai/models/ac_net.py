@@ -45,13 +45,16 @@ class ActorCriticNet(RLNet):
         if n > self.train_batch:
             self._grow_train_batch(n)
             self.train()
-        self._bind_optimizer(optimizer)
         dev = self._train.device
-        actions = torch.as_tensor(np.asarray(actions) if not torch.is_tensor(actions) else actions).to(dev, dtype=torch.int32)
+        actions = torch.as_tensor(np.asarray(actions) if not torch.is_tensor(actions) else actions)
         adv = torch.as_tensor(np.asarray(advantages, dtype=np.float32) if not torch.is_tensor(advantages) else advantages)
         adv = adv.to(dev, dtype=torch.float32)
         if actions.shape != (n,) or adv.shape != (n,):
             raise ValueError(f"policy_step: {n} positions, actions of shape {tuple(actions.shape)}, advantages of shape {tuple(adv.shape)}")
+        actions = self._train._per_row(actions, n, torch.int32, "policy_step: actions")
+        if bool((actions >= self.action_size).any()):
+            raise ValueError(f"policy_step: actions beyond the board's {self.action_size}")
+        self._bind_optimizer(optimizer)
         valid = _legal_moves(st)
         self._train_dirty = True
         logits = self._train.train_actor_forward(st)

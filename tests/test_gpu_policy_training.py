@@ -264,3 +264,16 @@ def test_loaded_parameters_end_an_actor_pass():
     c.train_load(sd)
     with pytest.raises(_hip.GoaiError, match="must follow"):
         c.train_actor_backward(torch.zeros(3, 26).cuda())
+
+
+def test_policy_step_checks_its_actions():
+    from go_ai.models import AdamW
+    net, _ = net_of(5, 1)
+    opt, st = AdamW(), np.zeros((2, 6, 5, 5), np.uint8)
+    before = {k: v.clone() for k, v in net.state_dict().items()}
+    for actions in ([0, 26], [0, 1 << 32], [0.0, 1.0], [True, False], torch.tensor([0, 26]).cuda(), torch.tensor([0.5, 1.0]).cuda()):
+        with pytest.raises(ValueError, match="actions"):
+            net.policy_step(opt, st, actions, [1.0, 1.0])
+    assert opt.params is None and all(torch.equal(before[k], v) for k, v in net.state_dict().items())
+    loss, _, _ = net.policy_step(opt, st, torch.tensor([-1, 25], dtype=torch.int8), [1.0, 1.0])
+    assert np.isfinite(loss) and opt.steps == 1
