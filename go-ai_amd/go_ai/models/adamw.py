@@ -64,8 +64,10 @@ class AdamW:
         if not n:
             raise ValueError("AdamW: no parameters")
         device = params[0].device
+        if ctx is not None and ctx.device != device:
+            raise ValueError(f"AdamW: parameters on {device}, a context of {ctx.device}")
         for p in params:
-            if p.device != device or p.dtype not in ELEM_TYPES or not p.is_contiguous():
+            if not p.is_cuda or p.device != device or p.dtype not in ELEM_TYPES or not p.is_contiguous():
                 raise ValueError("AdamW: parameters are contiguous float32, bfloat16 or float16 tensors of one GPU, got "
                                  f"{p.dtype} on {p.device}, strides {p.stride()}")
 

@@ -410,3 +410,16 @@ def test_refusals():
     loose = AdamW(None)
     with pytest.raises(RuntimeError, match="no parameters yet"):
         loose.step([])
+
+
+def test_parameters_of_another_device_than_the_context():
+    """The second GPU need not exist: a context that says it is there is enough."""
+    from types import SimpleNamespace
+    from go_ai.models import AdamW
+    p = tensors([(300,)], F32, 1)
+    with pytest.raises(ValueError, match="context"):
+        AdamW(p, ctx=SimpleNamespace(device=torch.device("cuda", 1)))
+    with pytest.raises(ValueError, match="context"):
+        AdamW().bind([torch.zeros(300)], SimpleNamespace(device=torch.device("cuda", 0)))
+    with pytest.raises(ValueError, match="GPU"):
+        AdamW().bind([torch.zeros(300)])

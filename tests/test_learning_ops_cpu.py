@@ -147,3 +147,14 @@ def test_action_types(dtype):
     least, most = np.iinfo(kind).min, np.iinfo(kind).max
     got = c._per_row(np.array([least, 5, most], kind), 3, torch.int32, "actions").tolist()
     assert got == [max(least, -1) if kind.itemsize == 8 else least, 5, min(most, 0x7fffffff)]
+
+
+def test_adamw_takes_no_host_tensors():
+    from types import SimpleNamespace
+
+    import torch
+    from go_ai.models import AdamW
+    with pytest.raises(ValueError, match="of one GPU"):
+        AdamW().bind([torch.zeros(300)])
+    with pytest.raises(ValueError, match="context"):
+        AdamW().bind([torch.zeros(300)], SimpleNamespace(device=torch.device("cuda", 0)))
