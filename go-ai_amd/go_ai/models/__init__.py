@@ -211,9 +211,9 @@ class RLNet:
 
     def _bind_optimizer(self, optimizer):
         """An AdamW without parameters of its own (or of this net's training state before it was rebuilt) takes this net's."""
-        if optimizer.params is not None and optimizer._ctx is self._train:
+        if optimizer._net is self and optimizer._ctx is self._train:
             return
-        if optimizer.params is not None and getattr(optimizer, "_net", None) is not self:
+        if optimizer.params is not None and optimizer._net is not self:
             raise ValueError("this AdamW already belongs to other parameters: a net needs one of its own (AdamW(None, ...))")
         if optimizer.params is not None:
             import warnings

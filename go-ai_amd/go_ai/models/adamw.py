@@ -44,7 +44,7 @@ class AdamW:
             raise ValueError("AdamW: max_norm must not be negative")
         self.steps = 0
         self.params = None
-        self._h = self._ctx = None
+        self._h = self._ctx = self._net = None
         params = None if params is None else list(params)
         if params and all(torch.is_tensor(p) and p.is_cuda for p in params):
             self.bind(params, ctx)
@@ -97,7 +97,8 @@ class AdamW:
             numels, _ctypes_table(ctypes.c_float, decays), self.state_bits, m.data_ptr() or scales.data_ptr(), v.data_ptr() or scales.data_ptr(),
             scales[0].data_ptr() if eight else None, scales[1].data_ptr() if eight else None, ctypes.byref(h)))
         self._h = h
-        self.params, self.device = params, device
+        self.params, self.device, self._net = params, device, None
+        self._addresses = [p.data_ptr() for p in params]
         self._gtypes, self._shapes, self._devices = gtypes, [p.shape for p in params], [device.index] * n
         self._m, self._v, self._scales, self._elems = m, v, scales, elems
         self._table = _ctypes_table(ctypes.c_void_p, [None] * n)
@@ -116,6 +117,11 @@ class AdamW:
             _hip.lib.goai_adamw_destroy(None if self._ctx.closed else self._ctx._h, self._h)
         self._h = None
 
+    def __getstate__(self):
+        if self._h is not None:
+            raise TypeError("AdamW: moments on the GPU are not copied or pickled; use state_dict")
+        return self.__dict__
+
     def __del__(self):
         try:
             self.close()
@@ -129,6 +135,8 @@ class AdamW:
 
     # ---- the step ----------------------------------------------------------------------------
     def _grads(self, grads):
+        if list(map(_address_of, self.params)) != self._addresses:
+            raise RuntimeError("AdamW: a parameter's memory was replaced since bind(): bind the optimiser again (fresh moments)")
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW: {len(self.params)} parameters, {len(grads)} gradients")
         try:                                                     # one pass per property: a third faster than tensor by tensor

@@ -423,3 +423,32 @@ def test_parameters_of_another_device_than_the_context():
         AdamW().bind([torch.zeros(300)], SimpleNamespace(device=torch.device("cuda", 0)))
     with pytest.raises(ValueError, match="GPU"):
         AdamW().bind([torch.zeros(300)])
+
+
+def test_a_bound_optimiser_is_not_copied():
+    import copy
+    import pickle
+    from go_ai.models import AdamW
+    p = tensors([(300,), (7,)], F32, 1)
+    opt = AdamW(p)
+    for f in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="state_dict"):
+            f(opt)
+
+
+def test_replaced_parameter_memory():
+    from go_ai.models import AdamW
+    p, g = tensors([(300,), (7,)], F32, 1), tensors([(300,), (7,)], F32, 2)
+    opt = AdamW(p)
+    opt.step(g)
+    old = p[0].data
+    p[0].data = old.clone()
+    before = old.clone()
+    with pytest.raises(RuntimeError, match="replaced"):
+        opt.step(g)
+    assert opt.steps == 1 and torch.equal(old, before) and torch.equal(p[0], before)
+    p[0].data = old
+    opt.step(g)
+    assert opt.steps == 2 and not torch.equal(p[0], before)
+    opt.bind(p)
+    assert opt.steps == 0 and not any(m.any() for m in opt.moments())

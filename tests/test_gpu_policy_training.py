@@ -277,3 +277,16 @@ def test_policy_step_checks_its_actions():
     assert opt.params is None and all(torch.equal(before[k], v) for k, v in net.state_dict().items())
     loss, _, _ = net.policy_step(opt, st, torch.tensor([-1, 25], dtype=torch.int8), [1.0, 1.0])
     assert np.isfinite(loss) and opt.steps == 1
+
+
+def test_an_optimiser_bound_elsewhere_is_not_a_nets():
+    """Bound by hand to other tensors, with the net's own context even, it has none of the net's gradients."""
+    from go_ai.models import AdamW
+    net, _ = net_of(5, 1)
+    st = np.zeros((2, 6, 5, 5), np.uint8)
+    opt = AdamW()
+    net.policy_step(opt, st, [0, 1], [1.0, 1.0])
+    for ctx in (net._train, None):
+        opt.bind([torch.zeros(10).cuda()], ctx)
+        with pytest.raises(ValueError, match="belongs"):
+            net.policy_step(opt, st, [0, 1], [1.0, 1.0])

@@ -158,3 +158,12 @@ def test_adamw_takes_no_host_tensors():
         AdamW().bind([torch.zeros(300)])
     with pytest.raises(ValueError, match="context"):
         AdamW().bind([torch.zeros(300)], SimpleNamespace(device=torch.device("cuda", 0)))
+
+
+def test_adamw_copies():
+    import copy
+    import pickle
+    from go_ai.models import AdamW
+    opt = AdamW(None, lr=0.25, max_norm=2.0)
+    for c in (copy.copy(opt), copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert c.lr == 0.25 and c.max_norm == 2.0 and c.params is None
