@@ -30,7 +30,7 @@ class AdamW:
     that is not finite leaves parameters and moments as they are; `norm` is the last step's norm (a GPU scalar).
 
     A step can be captured into a graph: step(grads, captured=True) reads lr and the bias corrections from GPU memory when it
-    runs; call advance() before the capture's first replay and before every further one."""
+    runs; call advance() before the capture's first replay and before every further one, on the stream that replays."""
 
     def __init__(self, params=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=0.0,
                  grad_dtype=None, ctx=None):
