@@ -15,6 +15,16 @@
 //      fraction bits, the largest r of the block is 1.0 = code 255; half a step: 2^-5 of r), 0 for r = 0.  A root that is not zero
 //      never becomes 0: m / (0 + eps) would throw the parameter away.
 // The update itself uses the moments before they are rounded.  A block whose largest value is below 2^-100 is held as zeros.
+//
+// Rounding them to the nearest code every step would lose every change below half a code, and with beta2 = 0.999 a step moves a root by
+// 0.05 % where half a code is 2^-5: a code would stand still while its block's largest root does and follow that one's scale
+// otherwise (elements whose gradients fall tenfold keep a v 80 times too large 7000 steps later; the other elements of a block whose largest
+// falls silent end at 0.13 of theirs), and a first moment of four steps of e4m3's smallest would stay for good.  So codes are rounded
+// at random, with the expectation right: the lower code's or the upper's, as often as the value is near to it.  A root then scatters about its own
+// value by sqrt(step / 2), 0.15 to 0.17 of it, with beta2's memory (v: 1/3), and its mean stays within a few percent.  The first AW_NEAREST = 16
+// steps after the moments were set go to the nearest, which has half the error: while 1 / t is at least half a code of e4m3 (2^-4) the newest
+// gradient's weight in fresh moments, (1 - beta) / (1 - beta^t) >= 1 / t, moves a code by itself, and 16 steps of loaded ones lose at most 16 of
+// those 0.05 %.  The random numbers are a hash of the step's number since then and the element: the same steps give the same bits.
 #include <float.h>
 #include <math.h>
 #include <string.h>
@@ -34,6 +44,7 @@ constexpr int AW_CHUNK = 2048;         // elements per workgroup: eight per thre
 constexpr int AW_LEVEL0 = 1777;        // (255 + AW_LEVEL0) << 19 is 1.0f
 constexpr float AW_SMALLEST = 0x1p-100f;
 constexpr int AW_LAUNCH = 256;         // tensors per launch: their gradients' addresses travel in the launch's arguments
+constexpr int AW_NEAREST = 16;         // steps whose 8-bit moments are rounded to the nearest (above)
 constexpr int AW_NORM_BLOCKS = 1024;   // workgroups (and float64 partial sums) of the norm (97 M: 599 us a step, with 512 or 2048 605)
 
 struct AwTensor {
@@ -55,6 +66,14 @@ struct AwGrads {
 struct AwScal {
     double lr;
     float b1, omb1, b2, omb2, eps, c1, c2;     // c1 = 1 / sqrt(1 - b2^t), c2 = lr / (1 - b1^t)
+    unsigned key;                              // of the step's random numbers
+    bool random;                               // 8-bit moments are rounded at random
+};
+// The GPU's count of steps, for those whose number the host does not know when they are launched: the replays of a captured one.
+struct AwClock {
+    long ticks;
+    unsigned key;
+    int random;
 };
 
 }  // namespace goai
@@ -65,8 +84,11 @@ struct goai_adamw {
     goai::AwState state{};
     std::vector<goai::AwTensor> tensors;
     std::vector<int> first;                    // first chunk of each tensor (and the total)
-    char* d_mem = nullptr;                     // one allocation: the norm's partial sums, tensors, chunks
+    long age = 0;                              // steps since the moments were set, those that the clock counts aside
+    bool ticking = false;                      // a step was captured: from then on the clock counts
+    char* d_mem = nullptr;                     // one allocation: the norm's partial sums, the clock, tensors, chunks
     double* d_partials = nullptr;              // AW_NORM_BLOCKS
+    goai::AwClock* d_clock = nullptr;
     goai::AwTensor* d_tensors = nullptr;
     goai::AwChunk* d_chunks = nullptr;
 };
@@ -130,7 +152,28 @@ template <int N> __device__ __forceinline__ void aw_sqrt(const float (&x)[N], fl
     }
 }
 
-// ---- moments in 8 bits: eight neighbouring codes per lane, a block on 32 lanes ----
+// ---- random numbers: a lane's eight elements take one word for their first moments and one for their roots, turned by four bits an
+// element (the top bits of two neighbours correlate by 1/16), as a bijection of every step's key each uniform by itself ----
+__host__ __device__ __forceinline__ unsigned aw_mix(unsigned x)
+{
+    x = (x ^ (x >> 16)) * 0x9E3779B1u;
+    x = (x ^ (x >> 15)) * 0x6A09E667u;
+    return x ^ (x >> 16);
+}
+__host__ __device__ __forceinline__ unsigned aw_key(long age) { return aw_mix((unsigned)age * 0x9E3779B9u + 0x7F4A7C15u); }
+
+struct AwRandom {
+    unsigned mean, root;
+};
+__device__ __forceinline__ AwRandom aw_random(unsigned key, long j)      // j: the first of a lane's eight elements
+{
+    AwRandom w;
+    w.mean = aw_mix((unsigned)(j >> 3) ^ key ^ ((unsigned)(j >> 35) * 0x9E3779B9u));
+    w.root = aw_mix(w.mean + 0x9E3779B9u);
+    return w;
+}
+
+// ---- moments in 8 bits: eight neighbouring codes per lane, a block on 32 lanes; `w`: rounded at random (nullptr: to the nearest) ----
 struct AwCodes {
     unsigned w[2];
 };
@@ -153,7 +196,7 @@ __device__ __forceinline__ void aw_root_of(AwCodes code, float scale, float (&r)
         r[k] = c ? __uint_as_float((c + AW_LEVEL0) << 19) * scale : 0.0f;
     }
 }
-__device__ __forceinline__ AwCodes aw_pack_mean(const float (&m)[8], float& scale)
+__device__ __forceinline__ AwCodes aw_pack_mean(const float (&m)[8], float& scale, const AwRandom* w = nullptr)
 {
     unsigned most = 0;
 #pragma unroll
@@ -162,7 +205,22 @@ __device__ __forceinline__ AwCodes aw_pack_mean(const float (&m)[8], float& scal
     const bool held = big >= AW_SMALLEST;
     const float inv = held ? (1.0f / big) * 448.0f : 0.0f;
     scale = held ? big * (1.0f / 448.0f) : 0.0f;
-    AwCodes c;
+    AwCodes c{ { 0, 0 } };
+    if (w) {
+        // (the conversion adds the top 20 bits of its random number in front of its cut.  The largest must not pass 448, above which the
+        // next code is NaN: the factor's two roundings are within 2^-22)
+        const float below = inv * (1.0f - 0x1p-22f);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            int x = 0;
+            x = __builtin_amdgcn_cvt_sr_fp8_f32(m[4 * h] * below, __builtin_rotateleft32(w->mean, 16 * h), x, 0);
+            x = __builtin_amdgcn_cvt_sr_fp8_f32(m[4 * h + 1] * below, __builtin_rotateleft32(w->mean, 16 * h + 4), x, 1);
+            x = __builtin_amdgcn_cvt_sr_fp8_f32(m[4 * h + 2] * below, __builtin_rotateleft32(w->mean, 16 * h + 8), x, 2);
+            x = __builtin_amdgcn_cvt_sr_fp8_f32(m[4 * h + 3] * below, __builtin_rotateleft32(w->mean, 16 * h + 12), x, 3);
+            c.w[h] = (unsigned)x;
+        }
+        return c;
+    }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(m[4 * h] * inv, m[4 * h + 1] * inv, 0, false);
@@ -170,7 +228,7 @@ __device__ __forceinline__ AwCodes aw_pack_mean(const float (&m)[8], float& scal
     }
     return c;
 }
-__device__ __forceinline__ AwCodes aw_pack_root(const float (&r)[8], float& scale)
+__device__ __forceinline__ AwCodes aw_pack_root(const float (&r)[8], float& scale, const AwRandom* w = nullptr)
 {
     unsigned most = 0;
 #pragma unroll
@@ -182,9 +240,11 @@ __device__ __forceinline__ AwCodes aw_pack_root(const float (&r)[8], float& scal
     AwCodes code{ { 0, 0 } };
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-        // to the nearest, ties to even, in units of the code; what is not zero is 1 at least (also where big is infinite)
+        // in units of the code: to the nearest, ties to even, or with 19 random bits in front of the cut; what is not zero is 1 at least
+        // (also where big is infinite)
         const int bits = __float_as_int(r[k] * inv);
-        const int c = (bits + (int)(0x3FFFFu - ((unsigned)AW_LEVEL0 << 19)) + ((bits >> 19) & 1)) >> 19;
+        const int up = w ? (int)(__builtin_rotateleft32(w->root, 4 * k) >> 13) : 0x3FFFF + ((bits >> 19) & 1);
+        const int c = (bits + up - (int)((unsigned)AW_LEVEL0 << 19)) >> 19;
         code.w[k / 4] |= (unsigned)min(max(c, (int)min(__float_as_uint(r[k]), 1u)), 255) << (8 * (k % 4));
     }
     return code;
@@ -225,8 +285,17 @@ __device__ __forceinline__ void aw_update8(const AwTensor& T, const AwState& S, 
     aw_math(p, g, m, v, root, s, k, keep);
     aw_store<PE, FULL>(T.p, i, T.n, p);
     float ms, vs;
-    *(AwCodes*)((char*)S.m + j) = aw_pack_mean(m, ms);
-    *(AwCodes*)((char*)S.v + j) = aw_pack_root(root, vs);
+    AwCodes cm, cv;
+    if (s.random) {
+        const AwRandom w = aw_random(s.key, j);
+        cm = aw_pack_mean(m, ms, &w);
+        cv = aw_pack_root(root, vs, &w);
+    } else {
+        cm = aw_pack_mean(m, ms);
+        cv = aw_pack_root(root, vs);
+    }
+    *(AwCodes*)((char*)S.m + j) = cm;
+    *(AwCodes*)((char*)S.v + j) = cv;
     if (j % AW_BLOCK == 0) {
         S.ms[j / AW_BLOCK] = ms;
         S.vs[j / AW_BLOCK] = vs;
@@ -274,7 +343,8 @@ __device__ __forceinline__ void aw_update(const AwTensor& T, const AwState& S, c
 
 template <int BITS>
 __global__ __launch_bounds__(256) void k_adamw(const AwTensor* __restrict__ tensors, const AwChunk* __restrict__ chunks, int base, AwState S,
-                                               AwGrads grads, AwScal s, const double* __restrict__ scal, const float* __restrict__ clip)
+                                               AwGrads grads, AwScal s, const double* __restrict__ scal, const float* __restrict__ clip,
+                                               const AwClock* __restrict__ clock)
 {
     // behind the norm, backwards: its last gradients are still in the memory-side cache (97 M elements: 599 -> 594 us)
     const AwChunk ch = chunks[clip ? gridDim.x - 1 - blockIdx.x : blockIdx.x];
@@ -288,6 +358,10 @@ __global__ __launch_bounds__(256) void k_adamw(const AwTensor* __restrict__ tens
         s.c1 = (float)scal[1];
         s.c2 = (float)scal[2];
     }
+    if (BITS == 8 && clock) {
+        s.key = clock->key;
+        s.random = clock->random != 0;
+    }
     const float keep = (float)(1.0 - s.lr * (double)T.decay);
     switch (T.ptype * 3 + T.gtype) {
         case 0: aw_update<BITS, 0, 0>(T, S, g, ch.chunk, s, k, keep); break;
@@ -300,6 +374,20 @@ __global__ __launch_bounds__(256) void k_adamw(const AwTensor* __restrict__ tens
         case 7: aw_update<BITS, 2, 1>(T, S, g, ch.chunk, s, k, keep); break;
         default: aw_update<BITS, 2, 2>(T, S, g, ch.chunk, s, k, keep); break;
     }
+}
+
+// before a step that the clock counts; `age`: the steps that it does not
+__global__ void k_adamw_tick(AwClock* clock, long age)
+{
+    if (threadIdx.x) return;
+    age += clock->ticks++;
+    clock->key = aw_key(age);
+    clock->random = age >= AW_NEAREST;
+}
+// the moments were set
+__global__ void k_adamw_restart(AwClock* clock, long age)
+{
+    if (threadIdx.x == 0) clock->ticks = -age;
 }
 
 // ---- the norm: float64 partial sums per workgroup, then one workgroup adds them in order (a launch of its own, 3 us: the last
@@ -453,13 +541,15 @@ static int aw_build(goai_adamw* o, int n, void* const* params, const int32_t* pt
         o->elems += aw_padded(numels[i]);
     }
     o->first.push_back((int)chunks.size());
-    const size_t pb = AW_NORM_BLOCKS * sizeof(double), tb = o->tensors.size() * sizeof(AwTensor), cb = chunks.size() * sizeof(AwChunk);
-    std::vector<char> image(pb + tb + cb);
+    const size_t nb = AW_NORM_BLOCKS * sizeof(double), pb = nb + sizeof(AwClock), tb = o->tensors.size() * sizeof(AwTensor),
+                 cb = chunks.size() * sizeof(AwChunk);
+    std::vector<char> image(pb + tb + cb);                                     // (zeros at first: the clock's)
     memcpy(image.data() + pb, o->tensors.data(), tb);
     if (cb) memcpy(image.data() + pb + tb, chunks.data(), cb);
     GOAI_HIP_CHECK(hipMalloc((void**)&o->d_mem, image.size()));
     GOAI_HIP_CHECK(hipMemcpy(o->d_mem, image.data(), image.size(), hipMemcpyHostToDevice));
     o->d_partials = (double*)o->d_mem;
+    o->d_clock = (AwClock*)(o->d_mem + nb);
     o->d_tensors = (AwTensor*)(o->d_mem + pb);
     o->d_chunks = (AwChunk*)(o->d_mem + pb + tb);
     return GOAI_OK;
@@ -553,12 +643,21 @@ int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, 
     }
     if (max_norm > 0.0 && (rc = aw_norm(c, o, grads, max_norm, clip))) return rc;
     AwScal s{ lr, (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
-              (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))), (float)(lr / (1.0 - pow(beta1, (double)t))) };
-    return aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
+              (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))), (float)(lr / (1.0 - pow(beta1, (double)t))), aw_key(o->age), o->age >= AW_NEAREST };
+    if (scalars) o->ticking = true;                // (it may be captured: its number is known when it runs)
+    const AwClock* clock = nullptr;
+    if (o->bits == 8 && o->ticking) {
+        k_adamw_tick<<<1, 64, 0, c->stream>>>(o->d_clock, o->age);
+        GOAI_HIP_CHECK(hipGetLastError());
+        clock = o->d_clock;
+    }
+    rc = aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
         if (n == 0) return;
-        if (o->bits == 32) k_adamw<32><<<n, 256, 0, c->stream>>>(o->d_tensors, chunks, base, o->state, g, s, scalars, clip);
-        else k_adamw<8><<<n, 256, 0, c->stream>>>(o->d_tensors, chunks, base, o->state, g, s, scalars, clip);
+        if (o->bits == 32) k_adamw<32><<<n, 256, 0, c->stream>>>(o->d_tensors, chunks, base, o->state, g, s, scalars, clip, clock);
+        else k_adamw<8><<<n, 256, 0, c->stream>>>(o->d_tensors, chunks, base, o->state, g, s, scalars, clip, clock);
     });
+    if (rc == GOAI_OK && !o->ticking) o->age++;
+    return rc;
 }
 
 int adamw_load_moments(goai_ctx* c, goai_adamw* o, const float* const* m, const float* const* v)
@@ -573,6 +672,10 @@ int adamw_load_moments(goai_ctx* c, goai_adamw* o, const float* const* m, const 
             if (n) kernel<<<n, 256, 0, c->stream>>>(o->d_tensors, chunks, base, o->state, g);
         });
     };
+    if (o->ticking) {
+        k_adamw_restart<<<1, 64, 0, c->stream>>>(o->d_clock, o->age);
+        GOAI_HIP_CHECK(hipGetLastError());
+    } else o->age = 0;
     const int rc = o->bits == 8 ? load(m, k_adamw_load<8, false>) : load(m, k_adamw_load<32, false>);
     if (rc) return rc;
     return o->bits == 8 ? load(v, k_adamw_load<8, true>) : load(v, k_adamw_load<32, true>);

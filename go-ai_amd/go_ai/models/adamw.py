@@ -24,7 +24,9 @@ class AdamW:
     params: contiguous tensors of one GPU (float32, bfloat16 or float16, in any mixture), or None / host tensors (what
     RLNet.parameters() yields): then the optimiser belongs to the net that it is first handed to (RLNet.optimize,
     RLNet.train_step), which gives it its parameters.  weight_decay and grad_dtype (None: each parameter's own type) are one value or
-    one per tensor.  state_bits = 8 holds the moments in a byte each, in blocks of 256 elements with a scale.
+    one per tensor.  state_bits = 8 holds the moments in a byte each, in blocks of 256 elements with a scale; from the 17th step after they
+    were set on they are rounded at random, so that changes below half a code add up (sqrt(v) scatters by about 0.15 of itself,
+    its mean follows float32's); the same steps give the same bits.
 
     step(grads) takes the gradients as a list in the parameters' order (None: that tensor stays as it is).  With max_norm a norm
     that is not finite leaves parameters and moments as they are; `norm` is the last step's norm (a GPU scalar).

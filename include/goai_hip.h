@@ -456,7 +456,10 @@ int64_t goai_adamw_state_elems(int n_tensors, const int64_t* numels);
  * gradients (GOAI_ELEM_*), sizes, weight decays.  The caller owns parameters and moments; they must outlive `out`.
  *   state_bits 32: exp_avg, exp_avg_sq float32 [elems];  avg_scales, sq_scales NULL
  *   state_bits 8:  exp_avg, exp_avg_sq uint8 [elems], avg_scales, sq_scales float32 [elems / 256]: codes and scales of the first
- *                  moment (e4m3) and of the second one's root, in blocks of 256 elements
+ *                  moment (e4m3) and of the second one's root (four fraction bits), in blocks of 256 elements.  A step rounds them at
+ *                  random, right in expectation (to the nearest a change below half a code would be lost, every step again): a
+ *                  root scatters by about 0.15 of its value; the first 16 steps after the moments were set go to the nearest.
+ *                  The random numbers follow from the step and the element alone: the same steps give the same bits.
  * The moments start as the caller left them (all zeros: a fresh optimiser); 16-byte aligned.  elems as above. */
 int goai_adamw_init(goai_ctx* ctx, int n_tensors, void* const* params, const int32_t* param_types, const int32_t* grad_types,
                     const int64_t* numels, const float* weight_decays, int state_bits, void* exp_avg, void* exp_avg_sq,
@@ -482,7 +485,7 @@ int goai_adamw_grad_norm(goai_ctx* ctx, goai_adamw* opt, const void* const* grad
 int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, int64_t t, double lr, double beta1, double beta2,
                     double eps, double max_norm, float* norm_and_coef, const double* scalars);
 
-/* Moments from float32 tensors (HOST tables of DEVICE pointers in the tensors' order; 8-bit ones are rounded to their codes). */
+/* Moments from float32 tensors (HOST tables of DEVICE pointers in the tensors' order; 8-bit ones are rounded to their nearest codes). */
 int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* const* exp_avg, const float* const* exp_avg_sq);
 /* Moments to float32 arrays [elems] of the flat layout (16-byte aligned): the values that 8-bit codes stand for. */
 int goai_adamw_moments(goai_ctx* ctx, goai_adamw* opt, float* exp_avg, float* exp_avg_sq);
