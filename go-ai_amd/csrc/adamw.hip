@@ -5,6 +5,9 @@
 //   m  = b1 m + (1 - b1) g',   v = b2 v + (1 - b2) g'^2
 //   p  = p (1 - lr wd) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
+// A step whose norm is not finite is skipped, and is no step of the bias corrections: t counts the others.  Only the GPU knows them in time, so
+// the corrections of a step that may be skipped, or that follows one, are computed there.
+//
 // All of it is float32, every operation rounded on its own (the library is built with -ffp-contract=off), so that a moment
 // in 8 bits is the same code wherever the step is computed.  The norm is summed in float64: a code next to the border of two
 // would follow the last bit of k.
@@ -69,11 +72,18 @@ struct AwScal {
     unsigned key;                              // of the step's random numbers
     bool random;                               // 8-bit moments are rounded at random
 };
-// The GPU's count of steps, for those whose number the host does not know when they are launched: the replays of a captured one.
+// The GPU's count of steps, for those whose number the host does not know when they are launched: the replays of a captured one, and
+// steps that are skipped when their gradients' norm is not finite.
 struct AwClock {
-    long ticks;
+    long ticks, skipped;                       // since the moments were set
+    double c1, c2;                             // the next step's (or the present one's)
     unsigned key;
     int random;
+};
+struct AwTick {
+    AwClock* clock;
+    long age, t;                               // steps that the clock does not count; this step's number, skipped ones counted
+    double lr, b1, b2;
 };
 
 }  // namespace goai
@@ -85,7 +95,7 @@ struct goai_adamw {
     std::vector<goai::AwTensor> tensors;
     std::vector<int> first;                    // first chunk of each tensor (and the total)
     long age = 0;                              // steps since the moments were set, those that the clock counts aside
-    bool ticking = false;                      // a step was captured: from then on the clock counts
+    bool ticking = false;                      // there was a step that the clock counts: from then on it counts all
     char* d_mem = nullptr;                     // one allocation: the norm's partial sums, the clock, tensors, chunks
     double* d_partials = nullptr;              // AW_NORM_BLOCKS
     goai::AwClock* d_clock = nullptr;
@@ -357,6 +367,9 @@ __global__ __launch_bounds__(256) void k_adamw(const AwTensor* __restrict__ tens
         s.lr = scal[0];
         s.c1 = (float)scal[1];
         s.c2 = (float)scal[2];
+    } else if (clock) {
+        s.c1 = (float)clock->c1;
+        s.c2 = (float)clock->c2;
     }
     if (BITS == 8 && clock) {
         s.key = clock->key;
@@ -376,18 +389,47 @@ __global__ __launch_bounds__(256) void k_adamw(const AwTensor* __restrict__ tens
     }
 }
 
-// before a step that the clock counts; `age`: the steps that it does not
-__global__ void k_adamw_tick(AwClock* clock, long age)
+// ---- the clock ----
+__device__ __forceinline__ double aw_c1(double b2, long t) { return 1.0 / sqrt(1.0 - pow(b2, (double)t)); }
+__device__ __forceinline__ double aw_c2(double lr, double b1, long t) { return lr / (1.0 - pow(b1, (double)t)); }
+__device__ __forceinline__ long aw_number(long t, const AwClock* clock) { return max(1L, t - clock->skipped); }
+
+__device__ __forceinline__ void aw_tick(const AwTick& k, bool skip)
 {
-    if (threadIdx.x) return;
-    age += clock->ticks++;
-    clock->key = aw_key(age);
-    clock->random = age >= AW_NEAREST;
+    if (skip) {
+        k.clock->skipped++;
+        return;
+    }
+    const long age = k.age + k.clock->ticks++;
+    k.clock->key = aw_key(age);
+    k.clock->random = age >= AW_NEAREST;
+}
+// before a step that the clock counts and whose norm, if it has one, was computed before
+__global__ __launch_bounds__(64) void k_adamw_tick(AwTick k, const float* __restrict__ clip)
+{
+    const long t = aw_number(k.t, k.clock);
+    if (threadIdx.x == 0) {
+        k.clock->c1 = aw_c1(k.b2, t);
+        k.clock->c2 = aw_c2(k.lr, k.b1, t);
+        aw_tick(k, clip && clip[1] != clip[1]);
+    }
 }
 // the moments were set
 __global__ void k_adamw_restart(AwClock* clock, long age)
 {
-    if (threadIdx.x == 0) clock->ticks = -age;
+    if (threadIdx.x == 0) {
+        clock->ticks = -age;
+        clock->skipped = 0;
+    }
+}
+// what a captured step of number t reads
+__global__ void k_adamw_scalars(AwTick k, double* __restrict__ out)
+{
+    if (threadIdx.x) return;
+    const long t = aw_number(k.t, k.clock);
+    out[0] = k.lr;
+    out[1] = aw_c1(k.b2, t);
+    out[2] = aw_c2(k.lr, k.b1, t);
 }
 
 // ---- the norm: float64 partial sums per workgroup, then one workgroup adds them in order (a launch of its own, 3 us: the last
@@ -436,17 +478,21 @@ __global__ __launch_bounds__(256) void k_adamw_sumsq(const AwTensor* __restrict_
     if (threadIdx.x == 0) partials[blockIdx.x] = add ? partials[blockIdx.x] + sum : sum;
 }
 
-// out[0] = norm, out[1] = the coefficient min(1, max_norm / norm); NaN where the norm is not finite
-__global__ __launch_bounds__(256) void k_adamw_norm(const double* __restrict__ partials, int n, double max_norm, float* __restrict__ out)
+// out[0] = norm, out[1] = the coefficient min(1, max_norm / norm); NaN where the norm is not finite.  With a clock it is a step's: the bias
+// corrections are another wavefront's while the partial sums are on their way.
+__global__ __launch_bounds__(256) void k_adamw_norm(const double* __restrict__ partials, int n, double max_norm, float* __restrict__ out, AwTick k)
 {
     __shared__ double lds[4];
     double sum = 0.0;
+    if (k.clock && threadIdx.x == 64) k.clock->c1 = aw_c1(k.b2, aw_number(k.t, k.clock));
+    if (k.clock && threadIdx.x == 128) k.clock->c2 = aw_c2(k.lr, k.b1, aw_number(k.t, k.clock));
     for (int i = threadIdx.x; i < n; i += 256) sum += partials[i];
     sum = aw_block_sum(sum, lds);
     if (threadIdx.x == 0) {
         const double norm = sqrt(sum);
         out[0] = (float)norm;
         out[1] = !(norm < (double)INFINITY) ? NAN : norm > max_norm ? (float)(max_norm / norm) : 1.0f;
+        if (k.clock) aw_tick(k, !(norm < (double)INFINITY));       // (behind the barriers: the others have read the clock)
     }
 }
 
@@ -610,14 +656,14 @@ static int aw_check_grads(goai_ctx* c, const goai_adamw* o, const void* const* g
     return GOAI_OK;
 }
 
-static int aw_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out)
+static int aw_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out, const AwTick& tick)
 {
     const int grid = std::max(1, std::min(AW_NORM_BLOCKS, o->first.back()));
     const int rc = aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
         k_adamw_sumsq<<<grid, 256, 0, c->stream>>>(o->d_tensors, chunks, n, base, g, o->d_partials, base != 0);
     });
     if (rc) return rc;
-    k_adamw_norm<<<1, 256, 0, c->stream>>>(o->d_partials, grid, max_norm, out);
+    k_adamw_norm<<<1, 256, 0, c->stream>>>(o->d_partials, grid, max_norm, out, tick);
     GOAI_HIP_CHECK(hipGetLastError());
     return GOAI_OK;
 }
@@ -625,7 +671,7 @@ static int aw_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double 
 int adamw_grad_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out)
 {
     const int rc = aw_check_grads(c, o, grads);
-    return rc ? rc : aw_norm(c, o, grads, max_norm, out);
+    return rc ? rc : aw_norm(c, o, grads, max_norm, out, AwTick{});
 }
 
 int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
@@ -641,15 +687,18 @@ int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, 
             return GOAI_ERR_STATE;
         }
     }
-    if (max_norm > 0.0 && (rc = aw_norm(c, o, grads, max_norm, clip))) return rc;
     AwScal s{ lr, (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps,
               (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))), (float)(lr / (1.0 - pow(beta1, (double)t))), aw_key(o->age), o->age >= AW_NEAREST };
-    if (scalars) o->ticking = true;                // (it may be captured: its number is known when it runs)
-    const AwClock* clock = nullptr;
-    if (o->bits == 8 && o->ticking) {
-        k_adamw_tick<<<1, 64, 0, c->stream>>>(o->d_clock, o->age);
+    // the clock counts steps that may be captured and steps that may be skipped, and once it has, all (scalars hold the corrections
+    // themselves: a captured step without 8-bit moments needs no clock)
+    if (scalars || clip) o->ticking = true;
+    const AwClock* clock = clip || (o->ticking && (o->bits == 8 || !scalars)) ? o->d_clock : nullptr;
+    const AwTick tick{ o->d_clock, o->age, (long)t, lr, beta1, beta2 };
+    if (max_norm > 0.0) {
+        if ((rc = aw_norm(c, o, grads, max_norm, clip, tick))) return rc;
+    } else if (clock) {
+        k_adamw_tick<<<1, 64, 0, c->stream>>>(tick, clip);
         GOAI_HIP_CHECK(hipGetLastError());
-        clock = o->d_clock;
     }
     rc = aw_launches(o, grads, [&](int base, const AwChunk* chunks, int n, const AwGrads& g) {
         if (n == 0) return;
@@ -658,6 +707,27 @@ int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, 
     });
     if (rc == GOAI_OK && !o->ticking) o->age++;
     return rc;
+}
+
+// scalars of step t for a captured step, less the steps skipped so far
+int adamw_scalars(goai_ctx* c, goai_adamw* o, int64_t t, double lr, double beta1, double beta2, double* scalars)
+{
+    GOAI_REQUIRE(o->device == c->device, "adamw: the optimiser lives on another GPU");
+    k_adamw_scalars<<<1, 64, 0, c->stream>>>(AwTick{ o->d_clock, 0, (long)t, lr, beta1, beta2 }, scalars);
+    GOAI_HIP_CHECK(hipGetLastError());
+    return GOAI_OK;
+}
+
+int adamw_skipped(goai_ctx* c, goai_adamw* o, int64_t* skipped)
+{
+    GOAI_REQUIRE(o->device == c->device, "adamw: the optimiser lives on another GPU");
+    *skipped = 0;
+    if (!o->ticking) return GOAI_OK;
+    long n = 0;
+    GOAI_HIP_CHECK(hipMemcpyAsync(&n, &o->d_clock->skipped, sizeof(n), hipMemcpyDeviceToHost, c->stream));
+    GOAI_HIP_CHECK(hipStreamSynchronize(c->stream));
+    *skipped = n;
+    return GOAI_OK;
 }
 
 int adamw_load_moments(goai_ctx* c, goai_adamw* o, const float* const* m, const float* const* v)

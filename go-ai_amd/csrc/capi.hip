@@ -628,18 +628,41 @@ int goai_adamw_grad_norm(goai_ctx* ctx, goai_adamw* opt, const void* const* grad
     return adamw_grad_norm(ctx, opt, grads, max_norm, norm_and_coef);
 }
 
-int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
-                    double max_norm, float* norm_and_coef, const double* scalars)
+static int check_adamw_step(int64_t t, double lr, double beta1, double beta2)
 {
     GOAI_REQUIRE(t >= 1, "adamw: the first step is t = 1");
     GOAI_REQUIRE(lr >= 0.0 && lr <= 1e30, "adamw: lr must be finite and not negative");
     GOAI_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw: betas must be in [0, 1)");
+    return GOAI_OK;
+}
+
+int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
+                    double max_norm, float* norm_and_coef, const double* scalars)
+{
+    const int rc = check_adamw_step(t, lr, beta1, beta2);
+    if (rc) return rc;
     GOAI_REQUIRE(eps >= 1e-30 && eps <= 1e30, "adamw: eps must be in 1e-30 .. 1e30");
     GOAI_REQUIRE(max_norm >= 0.0, "adamw: max_norm must not be negative");
     GOAI_REQUIRE(max_norm == 0.0 || norm_and_coef, "adamw: max_norm needs norm_and_coef");
     GOAI_REQUIRE(opt && grads, "NULL argument");
     CTX_ENTER(ctx);
     return adamw_step(ctx, opt, grads, t, lr, beta1, beta2, eps, max_norm, norm_and_coef, scalars);
+}
+
+int goai_adamw_scalars(goai_ctx* ctx, goai_adamw* opt, int64_t t, double lr, double beta1, double beta2, double* scalars)
+{
+    const int rc = check_adamw_step(t, lr, beta1, beta2);
+    if (rc) return rc;
+    GOAI_REQUIRE(opt && scalars, "NULL argument");
+    CTX_ENTER(ctx);
+    return adamw_scalars(ctx, opt, t, lr, beta1, beta2, scalars);
+}
+
+int goai_adamw_skipped(goai_ctx* ctx, goai_adamw* opt, int64_t* skipped)
+{
+    GOAI_REQUIRE(opt && skipped, "NULL argument");
+    CTX_ENTER(ctx);
+    return adamw_skipped(ctx, opt, skipped);
 }
 
 int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* const* exp_avg, const float* const* exp_avg_sq)

@@ -94,6 +94,8 @@ int adamw_destroy(goai_ctx* c, goai_adamw* o);
 int adamw_grad_norm(goai_ctx* c, goai_adamw* o, const void* const* grads, double max_norm, float* out);
 int adamw_step(goai_ctx* c, goai_adamw* o, const void* const* grads, int64_t t, double lr, double beta1, double beta2, double eps,
                double max_norm, float* clip, const double* scalars);
+int adamw_scalars(goai_ctx* c, goai_adamw* o, int64_t t, double lr, double beta1, double beta2, double* scalars);
+int adamw_skipped(goai_ctx* c, goai_adamw* o, int64_t* skipped);
 int adamw_load_moments(goai_ctx* c, goai_adamw* o, const float* const* m, const float* const* v);
 int adamw_moments(goai_ctx* c, goai_adamw* o, float* m, float* v);
 

@@ -90,6 +90,8 @@ _SIGNATURES = {
     "goai_adamw_destroy": [c_void_p, c_void_p],
     "goai_adamw_grad_norm": [c_void_p, c_void_p, c_void_p, c_double, c_void_p],
     "goai_adamw_step": [c_void_p, c_void_p, c_void_p, c_int64, c_double, c_double, c_double, c_double, c_double, c_void_p, c_void_p],
+    "goai_adamw_scalars": [c_void_p, c_void_p, c_int64, c_double, c_double, c_double, c_void_p],
+    "goai_adamw_skipped": [c_void_p, c_void_p, ctypes.POINTER(c_int64)],
     "goai_adamw_load_moments": [c_void_p, c_void_p, c_void_p, c_void_p],
     "goai_adamw_moments": [c_void_p, c_void_p, c_void_p, c_void_p],
     "goai_comm_unique_id": [c_void_p],

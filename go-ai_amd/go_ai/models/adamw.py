@@ -29,7 +29,8 @@ class AdamW:
     its mean follows float32's); the same steps give the same bits.
 
     step(grads) takes the gradients as a list in the parameters' order (None: that tensor stays as it is).  With max_norm a norm
-    that is not finite leaves parameters and moments as they are; `norm` is the last step's norm (a GPU scalar).
+    that is not finite skips the step: parameters and moments stay as they are, and it is not counted; `norm` is the last step's
+    norm (a GPU scalar).
 
     A step can be captured into a graph: step(grads, captured=True) reads lr and the bias corrections from GPU memory when it
     runs; call advance() before the capture's first replay and before every further one, on the stream that replays."""
@@ -44,7 +45,7 @@ class AdamW:
             raise ValueError("AdamW: state_bits must be 8 or 32")
         if not 0.0 <= self.max_norm:
             raise ValueError("AdamW: max_norm must not be negative")
-        self.steps = 0
+        self._calls = 0                                          # steps, skipped ones among them
         self.params = None
         self._h = self._ctx = self._net = None
         params = None if params is None else list(params)
@@ -110,7 +111,7 @@ class AdamW:
         for p in params:
             self.offsets.append(at)
             at += -(-p.numel() // BLOCK) * BLOCK
-        self.steps = 0
+        self._calls = 0
         return self
 
     def close(self):
@@ -136,6 +137,17 @@ class AdamW:
         self._ctx._bind()
 
     # ---- the step ----------------------------------------------------------------------------
+    @property
+    def steps(self):
+        """The number of steps behind the moments.  With max_norm this waits for the GPU, which knows the skipped ones."""
+        if self._h is None:
+            return self._calls
+        from .. import _hip
+        self._bound()
+        skipped = ctypes.c_int64()
+        _hip.check(_hip.lib.goai_adamw_skipped(self._ctx._h, self._h, ctypes.byref(skipped)))
+        return self._calls - skipped.value
+
     def _grads(self, grads):
         if list(map(_address_of, self.params)) != self._addresses:
             raise RuntimeError("AdamW: a parameter's memory was replaced since bind(): bind the optimiser again (fresh moments)")
@@ -161,26 +173,26 @@ class AdamW:
 
     def advance(self):
         """The next step's number; writes lr and the bias corrections of that step where a captured step reads them."""
+        from .. import _hip
         self._bound()
         if self._scalars is None:
             self._scalars = torch.zeros(3, dtype=torch.float64, device=self.device)
-        self.steps += 1
-        b1, b2 = self.betas
-        self._scalars.copy_(torch.tensor([self.lr, 1.0 / math.sqrt(1.0 - b2 ** self.steps), self.lr / (1.0 - b1 ** self.steps)],
-                                         dtype=torch.float64))
+        _hip.check(_hip.lib.goai_adamw_scalars(self._ctx._h, self._h, self._calls + 1, self.lr, self.betas[0], self.betas[1],
+                                               self._scalars.data_ptr()))
+        self._calls += 1
 
     def step(self, grads, captured=False):
-        """One step on the current stream; the number of the step is `steps` + 1 (captured: see advance)."""
+        """One step on the current stream: number `steps` + 1 (captured: see advance)."""
         from .. import _hip
         self._bound()
         table = self._grads(grads)
         if captured and self._scalars is None:
             raise RuntimeError("AdamW: call advance() before a captured step")
-        t = self.steps if captured else self.steps + 1
+        t = self._calls if captured else self._calls + 1
         _hip.check(_hip.lib.goai_adamw_step(self._ctx._h, self._h, table, max(t, 1), self.lr, self.betas[0], self.betas[1], self.eps,
                                             self.max_norm, self._clip.data_ptr() if self.max_norm else None,
                                             self._scalars.data_ptr() if captured else None))
-        self.steps = t
+        self._calls = t
 
     @property
     def norm(self):
@@ -221,7 +233,7 @@ class AdamW:
             held.append(given)
             tables.append(_ctypes_table(ctypes.c_void_p, list(map(_address_of, given))))
         _hip.check(_hip.lib.goai_adamw_load_moments(self._ctx._h, self._h, *tables))
-        self.steps = int(steps)
+        self._calls = int(steps)
 
     def state_dict(self):
         """steps and the moments as float32 host tensors in the parameters' order."""

@@ -475,15 +475,22 @@ int goai_adamw_grad_norm(goai_ctx* ctx, goai_adamw* opt, const void* const* grad
 /* Step number t (from 1): with g the gradient times the coefficient of norm_and_coef (DEVICE float[2]; NULL: 1; max_norm > 0: the
  * call computes it first, as goai_adamw_grad_norm does; max_norm = 0: it is as the caller left it),
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
- *   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in float32, rounded to the parameter's type and the moments' bits at the end.  A NaN coefficient leaves everything as it is,
- * a tensor without a gradient stays as it is.  A gradient whose
- * square is beyond float32 (|g| >= 2^64 after clipping) gives its element -- with 8 bits every element of its block that is not
- * zero -- an infinite second moment, which stays; one that is not finite spoils its element or block likewise.  scalars: NULL, or DEVICE double[3] = { lr, 1 / sqrt(1 - beta2^t), lr / (1 - beta1^t) },
- * read when the step runs, in place of lr and t: a step that is captured into a graph needs it (GOAI_ERR_STATE without), and the
- * graph's owner updates it between replays.  Two calls on the same optimiser must not run at the same time. */
+ *   p = p (1 - lr decay) - lr / (1 - beta1^n) * m / (sqrt(v) / sqrt(1 - beta2^n) + eps)
+ * in float32, rounded to the parameter's type and the moments' bits at the end.  A NaN coefficient skips the step: everything stays as it
+ * is.  t counts the calls; n is t less the steps skipped since the moments were set, which the GPU counts.  A tensor without a
+ * gradient stays as it is.  A gradient whose square is beyond float32 (|g| >= 2^64 after clipping) gives its element -- with 8
+ * bits every element of its block that is not zero -- an infinite second moment, which stays; one that is not finite spoils its
+ * element or block likewise.  scalars: NULL, or DEVICE double[3] = { lr, 1 / sqrt(1 - beta2^n), lr / (1 - beta1^n) } (written by
+ * goai_adamw_scalars), read when the step runs, in place of lr and t: a step that is captured into a graph needs it
+ * (GOAI_ERR_STATE without), and the graph's owner updates it between replays; the betas, eps and max_norm of a captured step are the
+ * capture's.  Gradients share no memory with parameters or moments.  Two calls on the same optimiser must not run at the same time. */
 int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, int64_t t, double lr, double beta1, double beta2,
                     double eps, double max_norm, float* norm_and_coef, const double* scalars);
+
+/* Writes the scalars of step number t for a captured step, the steps skipped so far taken off; asynchronous, on the stream that replays. */
+int goai_adamw_scalars(goai_ctx* ctx, goai_adamw* opt, int64_t t, double lr, double beta1, double beta2, double* scalars);
+/* The number of steps skipped since the moments were set, into *skipped (HOST); synchronises the stream if a step could be skipped. */
+int goai_adamw_skipped(goai_ctx* ctx, goai_adamw* opt, int64_t* skipped);
 
 /* Moments from float32 tensors (HOST tables of DEVICE pointers in the tensors' order; 8-bit ones are rounded to their nearest codes). */
 int goai_adamw_load_moments(goai_ctx* ctx, goai_adamw* opt, const float* const* exp_avg, const float* const* exp_avg_sq);
