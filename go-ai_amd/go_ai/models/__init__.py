@@ -209,12 +209,19 @@ class RLNet:
         self._train_dirty = True
         return self._train.train_params()
 
+    def _check_optimizer(self, optimizer):
+        """Whether an AdamW is this net's, or can become it."""
+        if optimizer.params is not None and optimizer._net is not self:
+            raise ValueError("this AdamW already belongs to other parameters: a net needs one of its own (AdamW(None, ...))")
+        types = optimizer.grad_dtype if isinstance(optimizer.grad_dtype, (list, tuple)) else [optimizer.grad_dtype]
+        if any(t not in (None, torch.float32) for t in types):
+            raise ValueError(f"AdamW: a net's gradients are float32, grad_dtype is {optimizer.grad_dtype}")
+
     def _bind_optimizer(self, optimizer):
         """An AdamW without parameters of its own (or of this net's training state before it was rebuilt) takes this net's."""
         if optimizer._net is self and optimizer._ctx is self._train:
             return
-        if optimizer.params is not None and optimizer._net is not self:
-            raise ValueError("this AdamW already belongs to other parameters: a net needs one of its own (AdamW(None, ...))")
+        self._check_optimizer(optimizer)
         if optimizer.params is not None:
             import warnings
             warnings.warn("go_ai.models: the training state was rebuilt: AdamW's moments were reset", RuntimeWarning)
@@ -234,6 +241,8 @@ class RLNet:
         next_states = children[actions] under random board symmetries, the actor (actor-critic net) argmax(pi) on
         states.  Returns (critic loss, critic accuracy, actor loss, actor accuracy), None where the net has no actor."""
         from .. import data
+        if isinstance(optimizer, AdamW):
+            self._check_optimizer(optimizer)
         self.train()
         children = np.asarray(children)
         bsz = len(children)
@@ -269,6 +278,8 @@ class RLNet:
         if sizes and min(sizes) < 2:
             raise ValueError(f"optimize: a batch of {min(sizes)} event(s); the optimisation step needs at least 2 "
                              "(BatchNorm over a batch); nothing was changed")
+        if isinstance(optimizer, AdamW):
+            self._check_optimizer(optimizer)
         if sizes and max(sizes) > self.train_batch:
             self._grow_train_batch(max(sizes))
         self.train()
