@@ -192,6 +192,24 @@ class RLNet:
                           RuntimeWarning)
         self.train_batch = int(n)
 
+    def reserve_train_batch(self, n, optimizer=None):
+        """Training buffers for batches of up to n events, before a step needs them.  Where that rebuilds them, an AdamW of this net
+        given here keeps its moments and step number (the reference's Adam starts again, with a warning)."""
+        if optimizer is not None:
+            self._check_optimizer(optimizer)
+        if n <= self.train_batch:
+            return
+        had = optimizer is not None and optimizer._net is self and optimizer._ctx is self._train
+        state = optimizer._carry() if had else None
+        self._grow_train_batch(n)
+        self.train()
+        if had:
+            import warnings
+            with warnings.catch_warnings():
+                warnings.simplefilter("ignore", category=RuntimeWarning)
+                self._bind_optimizer(optimizer)
+            optimizer._carry(state)
+
     def _tensor_shapes(self):
         return {k: tuple(v.shape) for k, v in self._sd.items() if not k.startswith("game_head.")}
 
@@ -216,6 +234,10 @@ class RLNet:
         types = optimizer.grad_dtype if isinstance(optimizer.grad_dtype, (list, tuple)) else [optimizer.grad_dtype]
         if any(t not in (None, torch.float32) for t in types):
             raise ValueError(f"AdamW: a net's gradients are float32, grad_dtype is {optimizer.grad_dtype}")
+        if optimizer._held is not None:
+            shapes = {k: s for k, s in self._tensor_shapes().items() if not k.endswith(("running_mean", "running_var"))}
+            held = optimizer._in_order(optimizer._held, list(shapes))
+            optimizer._check_moments(held["exp_avg"], held["exp_avg_sq"], list(shapes.values()), "the loaded state's")
 
     def _bind_optimizer(self, optimizer):
         """An AdamW without parameters of its own (or of this net's training state before it was rebuilt) takes this net's."""
@@ -224,17 +246,20 @@ class RLNet:
         self._check_optimizer(optimizer)
         if optimizer.params is not None:
             import warnings
-            warnings.warn("go_ai.models: the training state was rebuilt: AdamW's moments were reset", RuntimeWarning)
+            warnings.warn("go_ai.models: the training state was rebuilt: AdamW's moments were reset (reserve_train_batch keeps them)",
+                          RuntimeWarning)
         flat, grads = self._train.train_params(), self._train.train_grads()
-        params, optimizer._net_grads, optimizer._net_names = [], [], []
+        params, net_grads, names = [], [], []
         for k, shape in self._tensor_shapes().items():
             if not k.endswith(("running_mean", "running_var")):
                 off, n = self._train.train_parameter(k)
                 params.append(flat[off:off + n].view(shape))
-                optimizer._net_grads.append(grads[off:off + n].view(shape))
-                optimizer._net_names.append(k)
+                net_grads.append(grads[off:off + n].view(shape))
+                names.append(k)
+        if optimizer._held is not None:
+            optimizer._held = optimizer._in_order(optimizer._held, names)
         optimizer.bind(params, self._train)
-        optimizer._net = self
+        optimizer._net, optimizer._net_grads, optimizer._net_names = self, net_grads, names
 
     def train_step(self, optimizer, states, actions, reward, children, terminal, wins, pi):
         """One optimisation step on a batch of events (ac_net.py:67-86 / val_net.py:29-43): the critic learns -wins on

@@ -47,7 +47,7 @@ class AdamW:
             raise ValueError("AdamW: max_norm must not be negative")
         self._calls = 0                                          # steps, skipped ones among them
         self.params = None
-        self._h = self._ctx = self._net = None
+        self._h = self._ctx = self._net = self._held = None
         params = None if params is None else list(params)
         if params and all(torch.is_tensor(p) and p.is_cuda for p in params):
             self.bind(params, ctx)
@@ -59,7 +59,7 @@ class AdamW:
 
     # ---- parameters --------------------------------------------------------------------------
     def bind(self, params, ctx=None):
-        """Take these GPU tensors as the parameters; fresh moments."""
+        """Take these GPU tensors as the parameters; fresh moments, or those that load_state_dict left for them."""
         from .. import _hip
         from ..engine import ELEM_TYPES, Context
         params = list(params)
@@ -89,17 +89,20 @@ class AdamW:
         blocks = max(elems, 1) // BLOCK if self.state_bits == 8 else 0
         m, v = [torch.zeros(elems, dtype=state, device=device) for _ in range(2)]
         scales = torch.zeros((2, max(blocks, 1)), dtype=torch.float32, device=device)
-        self.close()
-        self._ctx = ctx if ctx is not None else Context(9, device.index)
-        self._ctx._bind()
+        held = self._held
+        if held is not None:
+            self._check_moments(held["exp_avg"], held["exp_avg_sq"], [p.shape for p in params], "the loaded state's")
+        ctx = ctx if ctx is not None else Context(9, device.index)
+        ctx._bind()
         h = ctypes.c_void_p()
         eight = self.state_bits == 8
         _hip.check(_hip.lib.goai_adamw_init(
-            self._ctx._h, n, _ctypes_table(ctypes.c_void_p, [p.data_ptr() for p in params]),
+            ctx._h, n, _ctypes_table(ctypes.c_void_p, [p.data_ptr() for p in params]),
             _ctypes_table(ctypes.c_int32, [ELEM_TYPES[p.dtype] for p in params]), _ctypes_table(ctypes.c_int32, [ELEM_TYPES[g] for g in gtypes]),
             numels, _ctypes_table(ctypes.c_float, decays), self.state_bits, m.data_ptr() or scales.data_ptr(), v.data_ptr() or scales.data_ptr(),
             scales[0].data_ptr() if eight else None, scales[1].data_ptr() if eight else None, ctypes.byref(h)))
-        self._h = h
+        self.close()                                             # (a refused bind leaves the optimiser as it was)
+        self._h, self._ctx, self._held = h, ctx, None
         self.params, self.device, self._net = params, device, None
         self._addresses = [p.data_ptr() for p in params]
         self._gtypes, self._shapes, self._devices = gtypes, [p.shape for p in params], [device.index] * n
@@ -112,6 +115,8 @@ class AdamW:
             self.offsets.append(at)
             at += -(-p.numel() // BLOCK) * BLOCK
         self._calls = 0
+        if held is not None:
+            self._load(held)
         return self
 
     def close(self):
@@ -141,7 +146,7 @@ class AdamW:
     def steps(self):
         """The number of steps behind the moments.  With max_norm this waits for the GPU, which knows the skipped ones."""
         if self._h is None:
-            return self._calls
+            return self._held["steps"] if self._held is not None else self._calls
         from .. import _hip
         self._bound()
         skipped = ctypes.c_int64()
@@ -212,19 +217,32 @@ class AdamW:
             _hip.check(_hip.lib.goai_adamw_moments(self._ctx._h, self._h, m.data_ptr(), v.data_ptr()))
         return m, v
 
+    def _carry(self, state=None):
+        """The moments as they are held, and the step number: out of here, or (to the same parameters in other memory) back in."""
+        self._bound()
+        if state is None:
+            return self.steps, self._m, self._v, self._scales
+        for mine, theirs in zip((self._m, self._v, self._scales), state[1:]):
+            mine.copy_(theirs)
+        self._calls = state[0]
+
     def _split(self, flat):
         return [flat[a:a + p.numel()].view(p.shape) for a, p in zip(self.offsets, self.params)]
+
+    @staticmethod
+    def _check_moments(exp_avg, exp_avg_sq, shapes, what):
+        if len(exp_avg) != len(shapes) or len(exp_avg_sq) != len(shapes):
+            raise ValueError(f"AdamW: {len(shapes)} parameters, {what} for {len(exp_avg)} and {len(exp_avg_sq)}")
+        for a, b, s in zip(exp_avg, exp_avg_sq, shapes):
+            if a.shape != s or b.shape != s:
+                raise ValueError(f"AdamW: a parameter of shape {tuple(s)}, {what} of shapes {tuple(a.shape)} and {tuple(b.shape)}")
 
     def load_moments(self, exp_avg, exp_avg_sq, steps):
         """Continue from these moments (one float tensor per parameter) after `steps` steps; 8-bit moments are rounded to their codes."""
         self._bound()
-        if len(exp_avg) != len(self.params) or len(exp_avg_sq) != len(self.params):
-            raise ValueError(f"AdamW: {len(self.params)} parameters, moments for {len(exp_avg)} and {len(exp_avg_sq)}")
         if int(steps) < 0:
             raise ValueError("AdamW: steps must not be negative")
-        for a, b, s in zip(exp_avg, exp_avg_sq, self._shapes):
-            if a.shape != s or b.shape != s:
-                raise ValueError(f"AdamW: a parameter of shape {tuple(s)}, moments of shapes {tuple(a.shape)} and {tuple(b.shape)}")
+        self._check_moments(exp_avg, exp_avg_sq, self._shapes, "moments")
         from .. import _hip
         tables, held = [], []
         for given in (exp_avg, exp_avg_sq):
@@ -236,9 +254,52 @@ class AdamW:
         self._calls = int(steps)
 
     def state_dict(self):
-        """steps and the moments as float32 host tensors in the parameters' order."""
+        """steps and the moments as float32 host tensors in the parameters' order, with the parameters' names if they are a net's; for
+        state_bits = 8 with their codes and scales too, which the values alone give back to some roundings only."""
+        if self._h is None and self._held is not None:
+            return dict(self._held)
         m, v = self.moments()
-        return {"steps": self.steps, "exp_avg": [x.cpu().clone() for x in self._split(m)], "exp_avg_sq": [x.cpu().clone() for x in self._split(v)]}
+        state = {"steps": self.steps, "exp_avg": [x.cpu().clone() for x in self._split(m)], "exp_avg_sq": [x.cpu().clone() for x in self._split(v)]}
+        if self.state_bits == 8:
+            state["codes"] = [[x.cpu().clone() for x in views] for views in self._codes()]
+        if self._net is not None:
+            state["names"] = list(self._net_names)
+        return state
+
+    def _codes(self):
+        """Views of the 8-bit moments' buffers by tensor: codes and scales of the first, codes and scales of the second."""
+        blocks = [(a // BLOCK, -(-p.numel() // BLOCK)) for a, p in zip(self.offsets, self.params)]
+        return [views for flat, scales in ((self._m, self._scales[0]), (self._v, self._scales[1]))
+                for views in ([flat[a:a + p.numel()] for a, p in zip(self.offsets, self.params)], [scales[a:a + n] for a, n in blocks])]
 
     def load_state_dict(self, state):
+        """Continue from a state_dict.  An optimiser that has no parameters yet keeps it for those that it is bound to: a net's AdamW
+        is resumed by loading its state before the net's next train_step, optimize or policy_step."""
+        if int(state["steps"]) < 0:
+            raise ValueError("AdamW: steps must not be negative")
+        if self._h is None:
+            self._held = {**state, "steps": int(state["steps"])}
+            return
+        if self._net is not None:
+            state = self._in_order(state, self._net_names)
+        self._load(state)
+
+    def _load(self, state):
         self.load_moments(state["exp_avg"], state["exp_avg_sq"], state["steps"])
+        if self.state_bits == 8 and "codes" in state:
+            for mine, theirs in zip(self._codes(), state["codes"]):
+                for a, b in zip(mine, theirs):
+                    a.copy_(b)
+
+    @staticmethod
+    def _in_order(state, names):
+        """A net's state in the order of `names`."""
+        if "names" not in state or list(state["names"]) == list(names):
+            return state
+        if sorted(state["names"]) != sorted(names):
+            raise ValueError("AdamW: the loaded state is of another net's parameters")
+        at = [list(state["names"]).index(k) for k in names]
+        turned = {**state, "names": list(names), **{k: [state[k][i] for i in at] for k in ("exp_avg", "exp_avg_sq")}}
+        if "codes" in state:
+            turned["codes"] = [[views[i] for i in at] for views in state["codes"]]
+        return turned
