@@ -7,7 +7,9 @@
 //
 // The forward pass reads the logits once: every lane keeps the maximum m of the logits it has seen and, with t = (x - m) c,
 // c = log2(e) / T, the sums l = sum 2^t and e = sum 2^t t; a maximum larger by d / c scales l by 2^-d and turns e into
-// 2^-d (e - d l).  All terms of e have one sign, so H = ln 2 (log2 l - e / l) loses nothing to cancellation.  Sums are float32.
+// 2^-d (e - d l).  All terms of e have one sign, so H = ln 2 (log2 l - e / l) loses nothing to cancellation.  Sums are float32; those over
+// the tiles of a long row carry what each addition rounded off (a lane's 2000 terms of 128001 equal columns, added one by one, were up to 3e-5
+// off: equal terms round the same way over and over).
 // A lane without columns has m = -FLT_MAX, l = e = 0: x - m is then never inf - inf, and l == 0 says that a row has no allowed
 // column.  t may be -inf (a column that is not allowed, or an overflow): its power is 0, and t is bounded in front of the product.
 #include <float.h>
@@ -49,6 +51,35 @@ __device__ __forceinline__ void lp_raise(LpStat& s, float m, LpFactor c)     // 
     s.e = f * fmaf(-d, s.l, s.e);
     s.l *= f;
     s.m = m;
+}
+
+// `low`: what the additions into s.l and s.e have rounded off (all of it where the sum is the larger of the two, as it is but for tiles behind
+// a raise)
+__device__ __forceinline__ void lp_raise(LpStat& s, LpStat& low, float m, LpFactor c)
+{
+    const float d = fminf(lp_times(m - s.m, c), 1000.0f), f = __builtin_amdgcn_exp2f(-d);
+    s.e = f * fmaf(-d, s.l, s.e);
+    low.e = f * fmaf(-d, low.l, low.e);
+    s.l *= f;
+    low.l *= f;
+    s.m = m;
+}
+__device__ __forceinline__ void lp_carry(float& sum, float& low, float x)
+{
+    const float y = x + low, t = sum + y;
+    low = y - (t - sum);
+    sum = t;
+}
+// a tile's columns (all <= s.m), summed four ways by themselves
+template <int N> __device__ __forceinline__ void lp_tile(LpStat& s, LpStat& low, const float (&x)[N], LpFactor c)
+{
+    LpStat a[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) a[k].m = s.m;
+#pragma unroll
+    for (int k = 0; k < N; k++) lp_add(a[k % 4], x[k], c);
+    lp_carry(s.l, low.l, (a[0].l + a[1].l) + (a[2].l + a[3].l));
+    lp_carry(s.e, low.e, (a[0].e + a[1].e) + (a[2].e + a[3].e));
 }
 
 // ---- cross-lane helpers: DPP moves within rows of 16 lanes and from row to row, which do without the LDS unit that shuffles go
@@ -460,7 +491,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
     const raw* p = (const raw*)A.x + row * A.xstride;
     const uint8_t* valid = A.valid ? A.valid + row * A.vstride : nullptr;
     const float given = splits == 1 ? lp_given<E>(A, row) : 0.0f;
-    LpStat s;
+    LpStat s, low;
     LpList t;
     float worst = -INFINITY;                               // the last alternative of the tiles before
     for (int base = c0 + (W == 4 ? wave : 0) * LP_TILE; base < c1; base += W * LP_TILE) {
@@ -494,9 +525,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void k
         float lane_max = -INFINITY;
 #pragma unroll
         for (int k = 0; k < LP_E; k++) lane_max = fmaxf(lane_max, x[k]);
-        lp_raise(s, fmaxf(s.m, lane_max), A.c2);
-#pragma unroll
-        for (int k = 0; k < LP_E; k++) lp_add(s, x[k], A.c2);
+        lp_raise(s, low, fmaxf(s.m, lane_max), A.c2);
+        lp_tile(s, low, x, A.c2);
         if constexpr (TOP) {
             if (__any(lane_max > worst)) {
                 const int last = A.cols - V;
