@@ -194,6 +194,9 @@ class Context:
 
     def _logits_and_mask(self, logits, valid):
         x, xs = self._rows(logits, "logits")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("logits that require a gradient: autograd does not see these calls; detach them (action_logprobs_grad has the "
+                             "gradient, for logits.backward)")
         if x.dtype not in ELEM_TYPES:
             if x.dtype != torch.float64:
                 raise ValueError(f"logits: float32, bfloat16 or float16 (float64 is rounded to float32), got {x.dtype}")
@@ -230,7 +233,7 @@ class Context:
     def action_logprobs(self, logits, actions=None, valid=None, temperature=1.0, top=0):
         """goai_action_logprobs: log probabilities of `actions` [rows] under softmax(logits / temperature) over the columns with
         valid != 0 (uint8 / bool, None: all), the entropy, the log of the sum, and the `top` best columns with their log
-        probabilities.  logits [rows, columns]: float32, bfloat16 or float16 on the GPU (any row stride; an expanded row or mask
+        probabilities.  Outside autograd's graph: logits that require a gradient are refused (detached ones are not).  logits [rows, columns]: float32, bfloat16 or float16 on the GPU (any row stride; an expanded row or mask
         is read as it is); host arrays are copied.  actions < 0: none."""
         self._bind()
         x, xs, v, vs = self._logits_and_mask(logits, valid)
@@ -259,7 +262,8 @@ class Context:
     def action_logprobs_grad(self, logits, actions, lse, entropy=None, d_logp=None, d_entropy=None, valid=None, temperature=1.0, out=None):
         """goai_action_logprobs_grad: the gradient with respect to the logits (a dense matrix in their type) of a loss whose
         gradients with respect to action_logprobs' logp and entropy are d_logp and d_entropy; lse and entropy are its outputs for
-        the same logits, valid and temperature.  out: a matrix to write into (the logits themselves, if nothing else reads them)."""
+        the same logits, valid and temperature.  out: a matrix to write into (the logits themselves, if nothing else reads them; autograd
+        counts it as changed in place)."""
         self._bind()
         x, xs, v, vs = self._logits_and_mask(logits, valid)
         rows, cols = x.shape
@@ -271,6 +275,10 @@ class Context:
         elif (out.dtype != x.dtype or tuple(out.shape) != (rows, cols) or out.device != self.device
               or (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols)):
             raise ValueError("out: a matrix of the logits' shape, type and device, its columns next to each other")
+        elif out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out: a tensor that requires a gradient would be changed in place")
+        else:
+            torch.autograd.graph.increment_version(out)
         if rows:
             p = _hip.dptr
             _hip.check(_hip.lib.goai_action_logprobs_grad(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), temperature, p(l), p(e), p(g),

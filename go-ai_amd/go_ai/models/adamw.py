@@ -105,6 +105,9 @@ class AdamW:
         self._h, self._ctx, self._held = h, ctx, None
         self.params, self.device, self._net = params, device, None
         self._addresses = [p.data_ptr() for p in params]
+        # autograd's counters of changes in place (views share their base's): a graph that saved a parameter before a step says so
+        bases = [p if p._base is None else p._base for p in params]
+        self._versions = list({id(b): b for b in bases}.values())
         self._gtypes, self._shapes, self._devices = gtypes, [p.shape for p in params], [device.index] * n
         self._m, self._v, self._scales, self._elems = m, v, scales, elems
         self._table = _ctypes_table(ctypes.c_void_p, [None] * n)
@@ -193,6 +196,7 @@ class AdamW:
         table = self._grads(grads)
         if captured and self._scalars is None:
             raise RuntimeError("AdamW: call advance() before a captured step")
+        torch.autograd.graph.increment_version(self._versions)
         t = self._calls if captured else self._calls + 1
         _hip.check(_hip.lib.goai_adamw_step(self._ctx._h, self._h, table, max(t, 1), self.lr, self.betas[0], self.betas[1], self.eps,
                                             self.max_norm, self._clip.data_ptr() if self.max_norm else None,
