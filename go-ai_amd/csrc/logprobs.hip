@@ -8,7 +8,7 @@
 // The forward pass reads the logits once: every lane keeps the maximum m of the logits it has seen and, with t = (x - m) c,
 // c = log2(e) / T, the sums l = sum 2^t and e = sum 2^t t; a maximum larger by d / c scales l by 2^-d and turns e into
 // 2^-d (e - d l).  All terms of e have one sign, so H = ln 2 (log2 l - e / l) loses nothing to cancellation.  Sums are float32; those over
-// the tiles of a long row carry what each addition rounded off (a lane's 2000 terms of 128001 equal columns, added one by one, were up to 3e-5
+// the tiles of a long row carry what each addition rounded off (a lane's 2000 terms of 128001 columns, added one by one, were up to 4e-5
 // off: equal terms round the same way over and over).
 // A lane without columns has m = -FLT_MAX, l = e = 0: x - m is then never inf - inf, and l == 0 says that a row has no allowed
 // column.  t may be -inf (a column that is not allowed, or an overflow): its power is 0, and t is bounded in front of the product.
@@ -713,7 +713,7 @@ struct LpGradArgs {
     const uint8_t* valid;
     long vstride;
     const int* actions;
-    float inv_t;
+    LpFactor inv_t;                        // as the forward pass has it: log p of the only column is 0 again
     const float *lse, *entropy, *g, *h;
     void* dx;
     long dstride;
@@ -758,7 +758,7 @@ template <int E, int L, int V> __global__ __launch_bounds__(256) void k_logprobs
     }
     const int a = A.actions ? A.actions[row] : -1;
     const float lse = A.lse[row], H = A.h ? A.entropy[row] : 0.0f, h = A.h ? A.h[row] : 0.0f;
-    const float g = a < 0 ? 0.0f : a >= A.cols ? NAN : A.g[row];
+    const float g = a < 0 ? 0.0f : a >= A.cols ? NAN : A.g[row], scale = A.inv_t.hi + A.inv_t.lo;
 #pragma unroll
     for (int q = 0; q < LG_N; q++) {
         const int c = c0 + (q * L + sub) * V, cc = min(c, last);
@@ -767,10 +767,10 @@ template <int E, int L, int V> __global__ __launch_bounds__(256) void k_logprobs
 #pragma unroll
         for (int k = 0; k < V; k++) {
             const float v = elem_to_float<E>(u[q].a[k]);
-            const float lp = __builtin_amdgcn_fmed3f(v * A.inv_t, -FLT_MAX, FLT_MAX) - lse, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+            const float lp = __builtin_amdgcn_fmed3f(lp_times(v, A.inv_t), -FLT_MAX, FLT_MAX) - lse, p = __builtin_amdgcn_exp2f(lp * LOG2E);
             // p log p is 0 at p = 0, also where log p is -inf
             const float t = fmaf(h, p * fmaxf(lp + H, -1000.0f), g * p);
-            d[k] = ok[q][k] && v != -INFINITY ? ((cc + k == a ? g : 0.0f) - t) * A.inv_t : 0.0f;
+            d[k] = ok[q][k] && v != -INFINITY ? ((cc + k == a ? g : 0.0f) - t) * scale : 0.0f;
         }
         if (c == cc) elem_store<E, V>(dx + c, d);
         else {
@@ -922,7 +922,7 @@ int launch_action_logprobs_grad(const void* logits, int elem, int64_t stride, co
                                 const int32_t* actions, double temperature, const float* lse, const float* entropy, const float* d_logp,
                                 const float* d_entropy, void* d_logits, int64_t d_stride, int64_t rows, int cols, hipStream_t st)
 {
-    LpGradArgs A{ logits, (long)stride, valid, (long)valid_stride, d_logp ? actions : nullptr, (float)(1.0 / temperature), lse, entropy, d_logp,
+    LpGradArgs A{ logits, (long)stride, valid, (long)valid_stride, d_logp ? actions : nullptr, lp_factor(1.0 / temperature), lse, entropy, d_logp,
                   d_entropy, d_logits, (long)d_stride, (long)rows, cols };
     LP_DISPATCH(elem, lp_launch_grad<E>(A, st));
     GOAI_HIP_CHECK(hipGetLastError());
