@@ -139,7 +139,7 @@ __device__ __forceinline__ float aw_max32(unsigned x)
 }
 
 // Square roots, correctly rounded: y = 1 / sqrt(x) to an ulp, s = x y, and one correction s + (x - s s) y / 2.  Against sqrtf it gives
-// the same for every x from 2^-102 on (all of them compared); sqrtf's own correction steps take twice the instructions.
+// the same for every x from 2^-102 on (the tests compare all significands); sqrtf's own correction steps take twice the instructions.
 // 0: y is held finite.  Smaller x, infinities and NaN: sqrtf.
 template <int N> __device__ __forceinline__ void aw_sqrt(const float (&x)[N], float (&s)[N])
 {

@@ -208,6 +208,14 @@ class AdamW:
         """The gradients' global norm at the last step with max_norm (before clipping): a GPU scalar."""
         return self._clip[0]
 
+    def grad_norm(self, grads):
+        """The global norm of these gradients (a GPU scalar), without a step: what a step with max_norm would clip."""
+        from .. import _hip
+        self._bound()
+        out = torch.empty(2, dtype=torch.float32, device=self.device)
+        _hip.check(_hip.lib.goai_adamw_grad_norm(self._ctx._h, self._h, self._grads(grads), math.inf, out.data_ptr()))
+        return out[0]
+
     # ---- moments -----------------------------------------------------------------------------
     def moments(self):
         """(exp_avg, exp_avg_sq) as flat float32 GPU tensors: tensor i's at [offsets[i] : offsets[i] + numel].  The optimiser's own
