@@ -626,7 +626,8 @@ int adamw_init(goai_ctx* c, int n, void* const* params, const int32_t* ptypes, c
 int adamw_destroy(goai_ctx* c, goai_adamw* o)
 {
     GOAI_REQUIRE(!c || o->device == c->device, "adamw: the optimiser lives on another GPU");
-    GOAI_HIP_CHECK(hipSetDevice(o->device));
+    OnDevice on_device;
+    GOAI_HIP_CHECK(on_device.enter(o->device));
     if (c) GOAI_HIP_CHECK(hipStreamSynchronize(c->stream));
     else GOAI_HIP_CHECK(hipDeviceSynchronize());
     aw_free(o);

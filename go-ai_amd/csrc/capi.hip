@@ -17,7 +17,8 @@ using namespace goai;
 
 #define CTX_ENTER(ctx)                                                   \
     GOAI_REQUIRE((ctx) != nullptr, "ctx is NULL");                       \
-    GOAI_HIP_CHECK(hipSetDevice((ctx)->device))
+    OnDevice on_device;                                                  \
+    GOAI_HIP_CHECK(on_device.enter((ctx)->device))
 
 extern "C" {
 
@@ -31,7 +32,8 @@ int goai_ctx_create(goai_ctx** out, int device, int board_size)
     int ndev = 0;
     GOAI_HIP_CHECK(hipGetDeviceCount(&ndev));
     GOAI_REQUIRE(device >= 0 && device < ndev, "no such GPU");
-    GOAI_HIP_CHECK(hipSetDevice(device));
+    OnDevice on_device;
+    GOAI_HIP_CHECK(on_device.enter(device));
     {
         const int rc = nn_static_setup(device);   // device address of goai_nn_forward_static's buffers, once per GPU
         if (rc) return rc;
@@ -50,7 +52,8 @@ int goai_ctx_create(goai_ctx** out, int device, int board_size)
 int goai_ctx_destroy(goai_ctx* ctx)
 {
     if (!ctx) return GOAI_OK;
-    (void)hipSetDevice(ctx->device);
+    OnDevice on_device;
+    (void)on_device.enter(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
     ctx->release();
     delete ctx;

@@ -24,6 +24,25 @@ void set_error(const std::string& msg);
         if (!(cond)) { ::goai::set_error(msg); return GOAI_ERR_ARG; }                         \
     } while (0)
 
+// A call works on its context's GPU and leaves the calling thread on the one that it was on.
+class OnDevice {
+    int before = -1;
+
+public:
+    hipError_t enter(int device)
+    {
+        int now = 0;
+        const hipError_t e = hipGetDevice(&now);
+        if (e != hipSuccess || now == device) return e;
+        before = now;
+        return hipSetDevice(device);
+    }
+    ~OnDevice()
+    {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
 inline bool size_supported(int s) { return s == 5 || s == 7 || s == 9 || s == 13 || s == 19; }
 
 // Dispatch a templated launcher on the board size.
