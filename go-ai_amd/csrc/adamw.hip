@@ -721,12 +721,15 @@ int adamw_scalars(goai_ctx* c, goai_adamw* o, int64_t t, double lr, double beta1
 
 int adamw_skipped(goai_ctx* c, goai_adamw* o, int64_t* skipped)
 {
-    GOAI_REQUIRE(o->device == c->device, "adamw: the optimiser lives on another GPU");
+    GOAI_REQUIRE(!c || o->device == c->device, "adamw: the optimiser lives on another GPU");
+    OnDevice on_device;
+    GOAI_HIP_CHECK(on_device.enter(o->device));
     *skipped = 0;
     if (!o->ticking) return GOAI_OK;
     long n = 0;
-    GOAI_HIP_CHECK(hipMemcpyAsync(&n, &o->d_clock->skipped, sizeof(n), hipMemcpyDeviceToHost, c->stream));
-    GOAI_HIP_CHECK(hipStreamSynchronize(c->stream));
+    if (c) GOAI_HIP_CHECK(hipStreamSynchronize(c->stream));
+    else GOAI_HIP_CHECK(hipDeviceSynchronize());
+    GOAI_HIP_CHECK(hipMemcpy(&n, &o->d_clock->skipped, sizeof(n), hipMemcpyDeviceToHost));
     *skipped = n;
     return GOAI_OK;
 }

@@ -664,7 +664,6 @@ int goai_adamw_scalars(goai_ctx* ctx, goai_adamw* opt, int64_t t, double lr, dou
 int goai_adamw_skipped(goai_ctx* ctx, goai_adamw* opt, int64_t* skipped)
 {
     GOAI_REQUIRE(opt && skipped, "NULL argument");
-    CTX_ENTER(ctx);
     return adamw_skipped(ctx, opt, skipped);
 }
 

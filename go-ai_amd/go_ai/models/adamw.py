@@ -151,9 +151,10 @@ class AdamW:
         if self._h is None:
             return self._held["steps"] if self._held is not None else self._calls
         from .. import _hip
-        self._bound()
         skipped = ctypes.c_int64()
-        _hip.check(_hip.lib.goai_adamw_skipped(self._ctx._h, self._h, ctypes.byref(skipped)))
+        if not self._ctx.closed:
+            self._ctx._bind()
+        _hip.check(_hip.lib.goai_adamw_skipped(None if self._ctx.closed else self._ctx._h, self._h, ctypes.byref(skipped)))
         return self._calls - skipped.value
 
     def _grads(self, grads):

@@ -489,7 +489,8 @@ int goai_adamw_step(goai_ctx* ctx, goai_adamw* opt, const void* const* grads, in
 
 /* Writes the scalars of step number t for a captured step, the steps skipped so far taken off; asynchronous, on the stream that replays. */
 int goai_adamw_scalars(goai_ctx* ctx, goai_adamw* opt, int64_t t, double lr, double beta1, double beta2, double* scalars);
-/* The number of steps skipped since the moments were set, into *skipped (HOST); synchronises the stream if a step could be skipped. */
+/* The number of steps skipped since the moments were set, into *skipped (HOST).  Synchronises the stream if a step could be skipped; ctx
+ * may be NULL once its context is gone (then the GPU). */
 int goai_adamw_skipped(goai_ctx* ctx, goai_adamw* opt, int64_t* skipped);
 
 /* Moments from float32 tensors (HOST tables of DEVICE pointers in the tensors' order; 8-bit ones are rounded to their nearest codes). */

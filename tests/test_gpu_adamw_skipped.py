@@ -194,3 +194,22 @@ def test_scalars():
     opt.advance()
     want = [3e-3, 1 / math.sqrt(1 - 0.99 ** 3), 3e-3 / (1 - 0.8 ** 3)]
     assert np.allclose(opt._scalars.cpu().numpy(), want, rtol=1e-14, atol=0) and opt.steps == 3
+
+
+def test_the_count_outlives_the_context():
+    """A net's training buffers are rebuilt under its optimiser: the number of steps can still be read."""
+    from go_ai.engine import Context
+    from go_ai.models import AdamW
+    for bad in (0, 2):
+        c = Context(9)
+        p = tensors(1)
+        opt = AdamW(p, max_norm=1.0, ctx=c)
+        for _ in range(3):
+            opt.step(tensors(2))
+        for _ in range(bad):
+            opt.step(spoil(tensors(3), math.nan))
+        c.close()
+        assert opt.steps == 3
+        with pytest.raises(RuntimeError, match="closed"):
+            opt.step(tensors(2))
+        assert opt.steps == 3
