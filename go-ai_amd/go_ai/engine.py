@@ -255,7 +255,7 @@ class Context:
             if cols > self.LOGPROBS_SHORT:              # few long rows are split, and the parts joined
                 need = _hip.lib.goai_action_logprobs_workspace(rows, cols, top)
                 work = torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None
-            _hip.check(_hip.lib.goai_action_logprobs(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), temperature, top, p(logp),
+            _hip.check(_hip.lib.goai_action_logprobs(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), float(temperature), top, p(logp),
                                                      p(entropy), p(lse), p(best), p(best_lp), rows, cols, p(work), need))
         return ActionLogprobs(logp, entropy, lse, best, best_lp)
 
@@ -281,7 +281,7 @@ class Context:
             torch.autograd.graph.increment_version(out)
         if rows:
             p = _hip.dptr
-            _hip.check(_hip.lib.goai_action_logprobs_grad(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), temperature, p(l), p(e), p(g),
+            _hip.check(_hip.lib.goai_action_logprobs_grad(self._h, p(x), ELEM_TYPES[x.dtype], xs, p(v), vs, p(a), float(temperature), p(l), p(e), p(g),
                                                           p(h), p(out), out.stride(0) if rows > 1 else cols, rows, cols))
         return out
 

@@ -40,7 +40,7 @@ class ActorCriticNet(RLNet):
         n = st.shape[0]
         if n < 2:
             raise ValueError(f"policy_step: {n} position(s); BatchNorm needs at least 2")
-        if not (1e-4 <= float(temperature) <= 1e4 and np.isfinite(float(entropy_weight))):
+        if not (1e-4 <= temperature <= 1e4 and np.isfinite(entropy_weight)):
             raise ValueError(f"policy_step: temperature {temperature} (1e-4 .. 1e4), entropy_weight {entropy_weight} (finite)")
         actions = torch.as_tensor(np.asarray(actions) if not torch.is_tensor(actions) else actions)
         adv = torch.as_tensor(np.asarray(advantages, dtype=np.float32) if not torch.is_tensor(advantages) else advantages.detach())
@@ -69,6 +69,7 @@ class ActorCriticNet(RLNet):
         if not isinstance(optimizer, AdamW):
             raise ValueError("policy_step: the optimizer must be a go_ai.models.AdamW")
         # all checks come before anything moves: parameters, moments, BatchNorm statistics, the training buffers
+        entropy_weight, temperature = float(entropy_weight), float(temperature)
         st, valid, actions, adv = self._policy_batch(states, actions, advantages, entropy_weight, temperature)
         self._check_optimizer(optimizer)
         n = st.shape[0]
@@ -80,7 +81,7 @@ class ActorCriticNet(RLNet):
         self._train_dirty = True
         logits = self._train.train_actor_forward(st)
         lp = self._train.action_logprobs(logits, actions, valid=valid, temperature=temperature)
-        d_entropy = torch.full((n,), -float(entropy_weight) / n, dtype=torch.float32, device=dev)
+        d_entropy = torch.full((n,), -entropy_weight / n, dtype=torch.float32, device=dev)
         d_logits = self._train.action_logprobs_grad(logits, actions, lp.lse, lp.entropy, adv * (-1.0 / n), d_entropy, valid=valid,
                                                     temperature=temperature, out=logits)
         self._train.train_actor_backward(d_logits)

@@ -186,7 +186,7 @@ class AdamW:
         self._bound()
         if self._scalars is None:
             self._scalars = torch.zeros(3, dtype=torch.float64, device=self.device)
-        _hip.check(_hip.lib.goai_adamw_scalars(self._ctx._h, self._h, self._calls + 1, self.lr, self.betas[0], self.betas[1],
+        _hip.check(_hip.lib.goai_adamw_scalars(self._ctx._h, self._h, self._calls + 1, float(self.lr), self.betas[0], self.betas[1],
                                                self._scalars.data_ptr()))
         self._calls += 1
 
@@ -199,7 +199,7 @@ class AdamW:
             raise RuntimeError("AdamW: call advance() before a captured step")
         torch.autograd.graph.increment_version(self._versions)
         t = self._calls if captured else self._calls + 1
-        _hip.check(_hip.lib.goai_adamw_step(self._ctx._h, self._h, table, max(t, 1), self.lr, self.betas[0], self.betas[1], self.eps,
+        _hip.check(_hip.lib.goai_adamw_step(self._ctx._h, self._h, table, max(t, 1), float(self.lr), self.betas[0], self.betas[1], self.eps,
                                             self.max_norm, self._clip.data_ptr() if self.max_norm else None,
                                             self._scalars.data_ptr() if captured else None))
         self._calls = t

@@ -88,3 +88,29 @@ def test_a_training_loop_with_autograd():
         theirs.step()
     for a, b in zip(net.parameters(), other.parameters()):
         assert np.allclose(a.detach().cpu().numpy(), b.detach().cpu().numpy(), rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("number", [np.float32, np.float64, torch.tensor, int])
+def test_numbers_of_other_types(ctx, number):
+    """Temperatures and learning rates as numpy or torch numbers, or whole ones."""
+    from go_ai.models import AdamW
+    from go_ai.models.ac_net import ActorCriticNet
+    x = torch.randn(5, 82, device="cuda")
+    a = torch.zeros(5, dtype=torch.int32, device="cuda")
+    want = ctx.action_logprobs(x, a, temperature=2.0)
+    assert torch.equal(ctx.action_logprobs(x, a, temperature=number(2)).logp, want.logp)
+    g = torch.ones(5, device="cuda")
+    assert torch.equal(ctx.action_logprobs_grad(x, a, want.lse, d_logp=g, temperature=number(2)),
+                       ctx.action_logprobs_grad(x, a, want.lse, d_logp=g, temperature=2.0))
+    p, q = torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+    opt, other = AdamW([p]), AdamW([q])
+    opt.lr, other.lr = number(2), 2.0
+    for o in (opt, other):
+        o.step([torch.ones(300, device="cuda")])
+    assert torch.equal(p, q) and p.any()
+    net, loss = ActorCriticNet(5, n_blocks=0, max_batch=4, train_batch=4), []
+    st = np.zeros((2, 6, 5, 5), np.uint8)
+    opt = AdamW(lr=0.0)
+    for t in (number(2), 2.0):
+        loss.append(net.policy_step(opt, st, [0, 1], [1.0, 1.0], entropy_weight=number(1), temperature=t))
+    assert loss[0] == loss[1]
