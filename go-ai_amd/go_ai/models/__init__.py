@@ -195,11 +195,11 @@ class RLNet:
     def reserve_train_batch(self, n, optimizer=None):
         """Training buffers for batches of up to n events, before a step needs them.  Where that rebuilds them, an AdamW of this net
         given here keeps its moments and step number (the reference's Adam starts again, with a warning)."""
-        if optimizer is not None:
+        if isinstance(optimizer, AdamW):
             self._check_optimizer(optimizer)
         if n <= self.train_batch:
             return
-        had = optimizer is not None and optimizer._net is self and optimizer._ctx is self._train
+        had = isinstance(optimizer, AdamW) and optimizer._net is self and optimizer._ctx is self._train and optimizer._h is not None
         state = optimizer._carry() if had else None
         self._grow_train_batch(n)
         self.train()
@@ -241,7 +241,7 @@ class RLNet:
 
     def _bind_optimizer(self, optimizer):
         """An AdamW without parameters of its own (or of this net's training state before it was rebuilt) takes this net's."""
-        if optimizer._net is self and optimizer._ctx is self._train:
+        if optimizer._net is self and optimizer._ctx is self._train and optimizer._h is not None:
             return
         self._check_optimizer(optimizer)
         if optimizer.params is not None:

@@ -303,6 +303,10 @@ class AdamW:
             for mine, theirs in zip(self._codes(), state["codes"]):
                 for a, b in zip(mine, theirs):
                     a.copy_(b)
+            # values that were changed since they were saved count, not the codes beside them
+            for mine, theirs in zip(self.moments(), (state["exp_avg"], state["exp_avg_sq"])):
+                if not all(torch.equal(a, b.to(self.device, dtype=torch.float32)) for a, b in zip(self._split(mine), theirs)):
+                    return self.load_moments(state["exp_avg"], state["exp_avg_sq"], state["steps"])
 
     @staticmethod
     def _in_order(state, names):

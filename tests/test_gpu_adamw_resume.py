@@ -213,3 +213,40 @@ def test_a_refused_bind_leaves_the_optimiser_as_it_was():
     assert opt.steps == 1 and all(torch.equal(a, b) for a, b in zip(before, opt.moments()))
     train(net, opt, (2,))
     assert opt.steps == 2
+
+
+def test_a_state_that_was_changed():
+    """Values that were edited after they were saved are loaded, not the codes that were saved beside them."""
+    from go_ai.models import AdamW
+    g = torch.Generator().manual_seed(1)
+    p = [torch.randn(700, generator=g).cuda(), torch.randn(4, 5, generator=g).cuda()]
+    opt = AdamW(p, state_bits=8)
+    for _ in range(3):
+        opt.step([torch.randn(x.shape, generator=g).cuda() for x in p])
+    saved = opt.state_dict()
+    codes = [x.clone() for x in (opt._m, opt._v, opt._scales)]
+    opt.step([torch.ones_like(x) for x in p])
+    opt.load_state_dict(saved)
+    assert all(torch.equal(a, b) for a, b in zip(codes, (opt._m, opt._v, opt._scales)))
+    for name, other in (("exp_avg", "exp_avg_sq"), ("exp_avg_sq", "exp_avg")):
+        state = opt.state_dict()
+        state[name] = [state[name][0], torch.zeros(4, 5)]
+        opt.load_state_dict(state)
+        got = opt.state_dict()
+        assert not got[name][1].any() and got[name][0].any() and got[other][1].any()
+        opt.load_state_dict(saved)
+
+
+def test_an_optimiser_that_was_closed():
+    """A net takes its closed AdamW as one without moments, and says so."""
+    from go_ai.models import Adam, AdamW
+    net, opt = net_of("ac", nn_ref.make_state_dict("ac", SIZE, 5, layers=1)), AdamW()
+    train(net, opt, (1, 2))
+    opt.close()
+    with pytest.warns(RuntimeWarning, match="reset"):
+        train(net, opt, (3,))
+    assert opt.steps == 1
+    opt.close()
+    net.reserve_train_batch(20, opt)
+    net.reserve_train_batch(21, Adam())
+    assert net.train_batch == 21
