@@ -263,7 +263,8 @@ __device__ __forceinline__ AwCodes aw_pack_root(const float (&r)[8], float& scal
 // ---- the step ----
 //
 // Bound by memory: 28 bytes an element in float32, 16 with moments in 8 bits, 10 with bfloat16 parameters and gradients too, at
-// some 55 vector instructions an element (39 T lane instructions a second: 1.4 ps, 10 bytes at 5 TB/s take 2).  The quotient is a
+// some 55 vector instructions an element, 60 with codes at random (39 T lane instructions a second: 1.5 ps, 10 bytes at 5 TB/s take 2;
+// 250 M elements 468 us to the nearest, 469 at random).  The quotient is a
 // product with the reciprocal (an ulp or two of the update).
 template <int N>
 __device__ __forceinline__ void aw_math(float (&p)[N], const float (&g)[N], float (&m)[N], float (&v)[N], float (&root)[N], const AwScal& s, float k,
