@@ -26,8 +26,8 @@
 // at random, with the expectation right: the lower code's or the upper's, as often as the value is near to it.  A root then scatters about its own
 // value by sqrt(step / 2), 0.15 to 0.17 of it, with beta2's memory (v: 1/3), and its mean stays within a few percent.  The first AW_NEAREST = 16
 // steps after the moments were set go to the nearest, which has half the error: while 1 / t is at least half a code of e4m3 (2^-4) the newest
-// gradient's weight in fresh moments, (1 - beta) / (1 - beta^t) >= 1 / t, moves a code by itself, and 16 steps of loaded ones lose at most 16 of
-// those 0.05 %.  The random numbers are a hash of the step's number since then and the element: the same steps give the same bits.
+// gradient's weight in fresh moments, (1 - beta) / (1 - beta^t) >= 1 / t, moves a code by itself, and 16 steps of loaded roots lose at most 16 of
+// those 0.05 % (of loaded first moments what 16 steps move them by, which the steps behind make up for).  The random numbers are a hash of the step's number since then and the element: the same steps give the same bits.
 #include <float.h>
 #include <math.h>
 #include <string.h>
